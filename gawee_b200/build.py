@@ -27,15 +27,18 @@ SOURCES = [
     "kernels/conv_gemm_tma.cu",
     "kernels/attention_tc.cu",
     "kernels/noalloc_gemm.cu",
+    "kernels/paged_kv.cu",
     "kernels/tc_probe.cu",
     "host/ir.cpp",
     "host/plan.cpp",
     "host/runtime.cpp",
+    "host/paged_kv.cpp",
 ]
 TOOLS = {
     "gawee-cuda-runner": "tools/gawee_cuda_runner.cpp",
 }
-HEADERS = ["kernels/kernels.h", "kernels/program.cuh", "kernels/tc_common.cuh", "host/ir.h", "host/plan.h", "host/launch.h", "host/npy.h"]
+HEADERS = ["kernels/kernels.h", "kernels/program.cuh", "kernels/tc_common.cuh", "kernels/paged_kv.h",
+           "kernels/paged_index.h", "host/ir.h", "host/plan.h", "host/launch.h", "host/npy.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",

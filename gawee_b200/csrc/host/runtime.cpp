@@ -1092,8 +1092,11 @@ gawee_status guard(gawee_ctx* ctx, F&& f) {
 
 const char* device_status_name(int st) {
   static const char* names[] = {"ok", "gather index out of range", "tensor-core barrier wait timed out",
-                                "invalid scalar program", "integer division by zero", "slice out of bounds"};
-  return st >= 0 && st < 6 ? names[st] : "error";
+                                "invalid scalar program", "integer division by zero", "slice out of bounds",
+                                "block table without a page for a cached row",
+                                "sequence longer than its block table, mask or weights",
+                                "token of a sequence outside the batch"};
+  return st >= 0 && st < 9 ? names[st] : "error";
 }
 
 // Reads and clears a device status word (after the work that writes it has
@@ -1151,6 +1154,7 @@ int value_info(const gawee::Value& v, int* dtype, int* rank, int64_t* shape) {
 namespace gawee {
 // Error text for calls without a context (creation, context-free entry points).
 void set_thread_error(const std::string& msg) { g_create_error = msg; }
+std::string device_status_text(int st) { return std::string("device reported: ") + device_status_name(st); }
 }  // namespace gawee
 
 extern "C" {

@@ -19,7 +19,7 @@ constexpr int kMaxInstr = 40;
 constexpr int kMaxRegs = 32;
 
 // Device-side dtype codes (same numbering as gawee::DType).
-enum DT : int8_t { DT_F32 = 0, DT_F64 = 1, DT_F16 = 2, DT_I64 = 3, DT_I32 = 4, DT_I1 = 5, DT_INDEX = 6 };
+enum DT : int8_t { DT_F32 = 0, DT_F64 = 1, DT_F16 = 2, DT_I64 = 3, DT_I32 = 4, DT_I1 = 5, DT_INDEX = 6, DT_BF16 = 7 };
 
 // Error codes written to the per-context device status word.
 enum Status : int {
@@ -29,6 +29,9 @@ enum Status : int {
   ST_BAD_PROGRAM = 3,      // elementwise program with an unknown opcode
   ST_INT_DIV_ZERO = 4,
   ST_SLICE_BOUNDS = 5,
+  ST_KV_PAGE = 6,      // a block table names no page for a cached row
+  ST_KV_LENGTH = 7,    // a sequence longer than its block table, mask or weights
+  ST_KV_SEQUENCE = 8,  // a token of a sequence outside the batch
 };
 
 struct DInstr {

@@ -1,0 +1,86 @@
+// Launch interfaces of the paged key/value cache kernels (paged_kv.cu).
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "kernels.h"
+#include "paged_index.h"
+
+namespace gawee {
+namespace kern {
+
+// Query heads of one key/value head that a block computes together; a larger
+// group takes several blocks, which read the same keys.
+constexpr int kKvHeadChunk = 8;
+
+// Rows of new tokens into the pages: token t's key k[t * k_stride + h * D ..]
+// goes to row positions[t] of sequence sequences[t] (nullptr: sequence t).  A
+// token with a negative position or sequence is left out.
+struct KvAppendParams {
+  PageGeom geom;
+  void *k_pages, *v_pages;
+  int page_dt;
+  const void *k, *v;
+  int dt;
+  int64_t k_stride, v_stride;
+  int64_t tokens;
+  const int32_t *sequences, *positions;
+  const int32_t* table;
+  int64_t table_stride, table_cols;
+  int batch;
+  int64_t last;  // nonzero: positions are lengths, the row is the last one; a length above `last` stores nothing
+  int* status;
+};
+cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t s);
+
+// Attention of one new token per sequence over its cached rows.
+struct KvAttendParams {
+  PageGeom geom;
+  void *k_pages, *v_pages;
+  int page_dt;
+  const void* q;
+  void* out;
+  int dt;  // of q, out, k and v
+  int64_t q_stride, out_stride;
+  int batch, heads;
+  float scale;
+  const int32_t* table;
+  int64_t table_stride, table_cols;
+  const int32_t* lengths;
+  int64_t max_len;  // a longer length is an error
+  const void *k, *v;  // the new token's row, stored first (nullptr: none)
+  int64_t k_stride, v_stride;
+  const float* mask;
+  int64_t mask_stride;
+  const float* weights;  // accumulators before (nullptr with weights_out set: zeros) ..
+  float* weights_out;    // .. and after this step (nullptr: not wanted)
+  int64_t w_stride, w_batch, wo_stride, wo_batch;
+  float* scores;         // [batch][heads][max_len], with weights_out
+  float* stats;          // [batch][heads][2]: maximum and sum, with weights_out
+  int* status;
+};
+cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s);
+
+// Eviction by accumulated weight.
+struct KvEvictParams {
+  PageGeom geom;
+  void *k_pages, *v_pages;
+  int page_dt;
+  const float* weights;
+  float* weights_out;
+  int64_t w_stride, w_batch, wo_stride, wo_batch;
+  const int32_t *table, *to_table;  // to_table nullptr: in place
+  int64_t table_stride, to_stride, table_cols, to_cols;
+  const int32_t* lengths;
+  int32_t* lengths_out;
+  int64_t max_len;
+  int batch, budget, recent;
+  int32_t* kept;     // [batch][kv_heads][budget]
+  int32_t* new_len;  // [batch] scratch
+  int* status;
+};
+cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t s);
+
+}  // namespace kern
+}  // namespace gawee

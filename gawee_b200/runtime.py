@@ -76,6 +76,12 @@ def load_library(path: str = LIB_PATH):
             "gawee_ciface_forward": (c.c_int, [P, P, c.POINTER(P), c.c_int]),
             "gawee_embedded_forward": (c.c_int, [c.c_char_p, c.c_int, P, c.POINTER(P), c.c_int]),
             "gawee_matmul_f32_noalloc": (c.c_int, [P, P, P, c.c_int64, c.c_int64, c.c_int64, P]),
+            "gawee_kv_create": (c.c_int, [P, c.c_int, c.POINTER(P)]),
+            "gawee_kv_destroy": (None, [P]),
+            "gawee_kv_append": (c.c_int, [P, P, P]),
+            "gawee_kv_attend": (c.c_int, [P, P, P]),
+            "gawee_kv_evict": (c.c_int, [P, P, P]),
+            "gawee_kv_synchronize": (c.c_int, [P, P]),
             "gawee_dp_unique_id": (c.c_int, [P]),
             "gawee_dp_init": (c.c_int, [P, c.c_int, c.c_int, P]),
             "gawee_dp_gather_output": (c.c_int, [P, c.c_int, P, P]),

@@ -51,7 +51,8 @@ enum {
   GAWEE_F16 = 2,
   GAWEE_I64 = 3,
   GAWEE_I32 = 4,
-  GAWEE_I1 = 5
+  GAWEE_I1 = 5,
+  GAWEE_BF16 = 7 /* paged key/value cache only; 6 is taken by the planner */
 };
 
 typedef struct gawee_ctx gawee_ctx;
@@ -211,6 +212,167 @@ gawee_status gawee_embedded_forward(const char* mlir_text, int device, void* res
  * ------------------------------------------------------------------------- */
 gawee_status gawee_matmul_f32_noalloc(const float* a, const float* b, float* c, int64_t m, int64_t n, int64_t k,
                                       void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged key/value cache (no counterpart in the reference, whose decode step
+ * concatenates the cache anew for each token and is compiled for one length).
+ *
+ * The keys and values of many sequences lie in pages of page_size rows, two
+ * arrays [num_pages][kv_heads][page_size][head_dim] of f32, f16 or bf16 that
+ * the caller owns (one pair per layer).  A block table, int32 [batch][columns]
+ * on the device, names each sequence's pages in order: row i of sequence b is
+ * slot i % page_size of page table[b][i / page_size].  Columns behind a
+ * sequence's last row are never read.  Lengths and tables are read on the
+ * device when the call runs, so that one captured call serves every step.
+ *
+ * A gawee_kv handle holds the shapes and the scratch memory, allocated once;
+ * one handle serves any number of layers.
+ *   - Every pointer is device memory of the handle's device; activations (q,
+ *     out, k, v) are of one type, f32, f16 or bf16, whatever the pages' type.
+ *     Pages are 16-byte aligned, and so is the distance between two pages.
+ *     Arrays of a call do not overlap unless a call says so.
+ *   - Calls enqueue on `stream` (NULL: the device's default stream), do not
+ *     wait, allocate nothing and can be captured into a graph.  They leave the
+ *     calling thread's current device as it was.
+ *   - Calls on one handle share its scratch: they are ordered by the caller,
+ *     by one stream or by events; replays of graphs that hold them too.  Calls
+ *     that may run at the same time take a handle each.
+ *   - A bad argument is refused with GAWEE_ERR_INVALID before anything is
+ *     enqueued; the message is read with gawee_last_error(NULL, ...).
+ *   - What only the device can see (a table entry that names no page, a length
+ *     beyond the table) is recorded in the handle, and gawee_kv_synchronize
+ *     returns GAWEE_ERR_DEVICE; memory outside the arrays is not touched.
+ * ------------------------------------------------------------------------- */
+typedef struct gawee_kv gawee_kv;
+
+typedef struct {
+  int dtype;           /* of the pages: GAWEE_F32, GAWEE_F16 or GAWEE_BF16 */
+  int heads;           /* query heads, a multiple of kv_heads: query head h reads key/value head h / (heads / kv_heads) */
+  int kv_heads;
+  int head_dim;        /* a multiple of 8, up to 256 */
+  int page_size;       /* rows of a page, up to 65536 */
+  int64_t num_pages;
+  int64_t page_stride; /* elements between pages; 0: kv_heads * page_size * head_dim */
+  int max_batch;       /* sequences of a call at most, up to 65535 */
+  int max_pages;       /* columns of a block table at most */
+  int weights;         /* nonzero: gawee_kv_attend may return attention weights (scratch of
+                          max_batch * heads * max_pages * page_size floats) */
+} gawee_kv_desc;
+
+/* device -1: a handle without a device, whose calls check their arguments and
+ * then return GAWEE_ERR_CUDA (as gawee_plan_text plans without one). */
+gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** out);
+void gawee_kv_destroy(gawee_kv* kv); /* waits for the device's work first */
+
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  const void* k; /* new rows [tokens][kv_heads][head_dim], stored rounded to nearest in the pages' type */
+  const void* v;
+  int dtype;        /* of k and v */
+  int64_t k_stride; /* elements between tokens; a column slice of a wider projection is fine */
+  int64_t v_stride;
+  int64_t tokens;
+  const int32_t* sequences; /* [tokens]: row of the block table; NULL: token t is of sequence t */
+  const int32_t* positions; /* [tokens]: row within the sequence */
+  const int32_t* block_table;
+  int64_t table_stride; /* elements between rows */
+  int table_cols;
+  int batch; /* rows of the block table */
+} gawee_kv_append_args;
+
+/* Write the rows of new tokens (a prompt, or one token per sequence) into the
+ * pages.  Tokens with a negative sequence or position are left out.  Two
+ * tokens of one call that name the same row leave one of the two there. */
+gawee_status gawee_kv_append(gawee_kv* kv, const gawee_kv_append_args* args, void* stream);
+
+typedef struct {
+  void* k_pages; /* written only where k and v are given */
+  void* v_pages;
+  const void* q; /* [batch][heads][head_dim] */
+  void* out;     /* [batch][heads][head_dim] */
+  int dtype;     /* of q, out, k and v */
+  int64_t q_stride; /* elements between sequences */
+  int64_t out_stride;
+  int batch;
+  float scale; /* of the scores: 1 / sqrt(head_dim) as a rule */
+  const int32_t* block_table;
+  int64_t table_stride;
+  int table_cols;
+  const int32_t* lengths; /* [batch]: cached rows, the new token's own among them */
+  const void* k; /* optional, with v: [batch][kv_heads][head_dim], the new token's rows */
+  const void* v;
+  int64_t k_stride;
+  int64_t v_stride;
+  const float* mask; /* optional: [batch][mask_cols], added to the scaled scores */
+  int64_t mask_stride;
+  int64_t mask_cols;
+  const float* weights; /* optional: [batch][kv_heads][weights_cols], accumulated attention weights */
+  int64_t weights_stride;       /* elements between heads */
+  int64_t weights_batch_stride; /* elements between sequences */
+  float* weights_out;           /* the same after this step; may be `weights` itself */
+  int64_t weights_out_stride;
+  int64_t weights_out_batch_stride;
+  int64_t weights_cols;
+} gawee_kv_attend_args;
+
+/* Attention of one new token per sequence over its rows 0 .. length - 1:
+ *   out[b][h] = sum_i p_i V_i,  p = softmax_i(scale * (q[b][h] . K_i) + mask[b][i]),
+ * with fp32 scores, maxima and sums.  With k and v, they are first stored as
+ * row length - 1 (rounded to the pages' type, and attended as stored); the
+ * page of that row then belongs to this sequence alone.  With weights_out,
+ * each row's weights, summed over the query heads that share its key/value
+ * head, are added: weights_out = weights + sum_h p_h (weights NULL: zeros);
+ * columns from length on are not touched.
+ *   - A mask value of -inf takes the row out, whatever its K and V hold.  Other
+ *     values are added as they are: a mask of the lowest finite value is one.
+ *     A sequence of length 0, or whose rows are all taken out, gives zeros.
+ *   - A negative length marks a batch row without a sequence: its rows of out,
+ *     weights_out and the pages are left as they were.
+ *   - The same call gives the same bits: partial sums are joined in a fixed
+ *     order, which depends on the shapes and the lengths of the batch. */
+gawee_status gawee_kv_attend(gawee_kv* kv, const gawee_kv_attend_args* args, void* stream);
+
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  const float* weights; /* [batch][kv_heads][weights_cols], as accumulated by gawee_kv_attend */
+  int64_t weights_stride;
+  int64_t weights_batch_stride;
+  float* weights_out; /* of the kept rows, at their new places; may be `weights` itself */
+  int64_t weights_out_stride;
+  int64_t weights_out_batch_stride;
+  int64_t weights_cols;
+  int batch;
+  const int32_t* block_table;
+  int64_t table_stride;
+  int table_cols;
+  const int32_t* to_table; /* NULL: in place; else [batch][to_cols], the pages that receive the kept rows */
+  int64_t to_stride;
+  int to_cols;
+  const int32_t* lengths;
+  int32_t* lengths_out; /* may be `lengths` itself */
+  int budget;           /* rows that a sequence keeps at most, at least 1 */
+  int recent;           /* of these, the last rows that always stay, 0 .. budget */
+  int32_t* kept;        /* [batch][kv_heads][budget]: earlier positions of the kept rows, ascending; -1 behind them */
+} gawee_kv_evict_args;
+
+/* Cut sequences longer than `budget` down to it.  Each key/value head keeps
+ * the last `recent` rows and, of the others, the budget - recent of greatest
+ * weight (equal weights: the lowest position; NaN below every number).  Kept rows move, in
+ * order, to rows 0 .. budget - 1; their weights too, and weights_out from there to
+ * the old length becomes 0; lengths_out = min(length, budget).  Sequences
+ * within the budget keep every row.
+ *   - In place, a sequence's pages belong to it alone; those behind the budget
+ *     are free afterwards.  With to_table, all kept rows are copied into its
+ *     pages, which are no sequence's pages in block_table: pages shared between sequences stay whole.
+ *   - A negative length marks a batch row without a sequence: its kept is -1, its
+ *     length is passed on, nothing else is touched. */
+gawee_status gawee_kv_evict(gawee_kv* kv, const gawee_kv_evict_args* args, void* stream);
+
+/* Wait for `stream` and check the handle's status word: GAWEE_ERR_DEVICE if a
+ * call flagged an error since the last check. */
+gawee_status gawee_kv_synchronize(gawee_kv* kv, void* stream);
 
 /* Diagnostic: the tensor cores' TF32 rate on `device`, measured now (one CTA
  * per SM issuing back-to-back M = 128, N = 128, K = 8 tcgen05 TF32 MMAs with
