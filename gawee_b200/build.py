@@ -28,6 +28,9 @@ SOURCES = [
     "kernels/attention_tc.cu",
     "kernels/noalloc_gemm.cu",
     "kernels/paged_kv.cu",
+    "kernels/paged_attend_f32.cu",
+    "kernels/paged_attend_f16.cu",
+    "kernels/paged_attend_bf16.cu",
     "kernels/tc_probe.cu",
     "host/ir.cpp",
     "host/plan.cpp",
@@ -38,7 +41,7 @@ TOOLS = {
     "gawee-cuda-runner": "tools/gawee_cuda_runner.cpp",
 }
 HEADERS = ["kernels/kernels.h", "kernels/program.cuh", "kernels/tc_common.cuh", "kernels/paged_kv.h",
-           "kernels/paged_index.h", "host/ir.h", "host/plan.h", "host/launch.h", "host/npy.h"]
+           "kernels/paged_index.h", "kernels/paged_common.cuh", "kernels/paged_attend.cuh", "host/ir.h", "host/plan.h", "host/launch.h", "host/npy.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",

@@ -22,16 +22,24 @@ struct gawee_kv {
   int32_t* new_len = nullptr;  // [max_batch]
   float* stats = nullptr;      // [max_batch][heads][2], with desc.weights
   float* scores = nullptr;     // [max_batch][heads][max_pages * page_size], with desc.weights
+  float* parts = nullptr;      // attend's partial states
+  unsigned* arrived = nullptr; // attend's counters, 0 between calls
+  int sms = 0;
   ~gawee_kv() {
     cudaFree(status);
     cudaFree(new_len);
     cudaFree(stats);
     cudaFree(scores);
+    cudaFree(parts);
+    cudaFree(arrived);
   }
 };
 
 namespace {
 
+using gawee::kern::kKvHeadsLeast;
+using gawee::kern::kKvHeadsMost;
+using gawee::kern::kKvMaxBlocksPerSm;
 using gawee::kern::PageGeom;
 
 gawee_status fail(gawee_status st, const std::string& what) {
@@ -161,6 +169,13 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     if (e == cudaSuccess && d.weights) e = cudaMalloc((void**)&kv->stats, sizeof(float) * 2 * rows);
     if (e == cudaSuccess && d.weights)
       e = cudaMalloc((void**)&kv->scores, sizeof(float) * rows * d.max_pages * d.page_size);
+    const int group = d.heads / d.kv_heads, block_heads = group > kKvHeadsLeast ? kKvHeadsMost : kKvHeadsLeast;
+    const size_t counters = (size_t)d.max_batch * d.kv_heads * ((group + kKvHeadsLeast - 1) / kKvHeadsLeast);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess)
+      e = cudaMalloc((void**)&kv->parts, sizeof(float) * 2 * kv->sms * kKvMaxBlocksPerSm * block_heads * (d.head_dim + 2));
+    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->arrived, sizeof(unsigned) * counters);
+    if (e == cudaSuccess) e = cudaMemset(kv->arrived, 0, sizeof(unsigned) * counters);
     if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
@@ -296,6 +311,10 @@ gawee_status gawee_kv_attend(gawee_kv* kv, const gawee_kv_attend_args* a, void* 
     p.wo_batch = a->weights_out_batch_stride;
     p.scores = kv->scores;
     p.stats = kv->stats;
+    p.parts = kv->parts;
+    p.arrived = kv->arrived;
+    p.device = kv->device;
+    p.sms = kv->sms;
     p.status = kv->status;
     return run_on(kv, kName, [&] { return launch_kv_attend(p, static_cast<cudaStream_t>(stream)); });
   });

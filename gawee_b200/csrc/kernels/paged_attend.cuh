@@ -1,0 +1,891 @@
+// Attention of one new token per sequence over a paged key/value cache.
+//
+//   s_i = scale * (q . K_i) + mask_i,  p = softmax(s),  out = sum_i p_i V_i
+//
+// Every cached byte is read once and takes part in a few operations, so the
+// bound is HBM bandwidth (with few query heads to a key/value head) and the
+// kernel is built to keep loads in flight:
+//
+//   * The keys of a (sequence, key/value head, chunk of query heads) segment
+//     are cut into tiles, and all tiles of the batch, in order, are divided
+//     evenly over a fixed grid of resident blocks: a block takes a contiguous
+//     run of tiles, whatever the lengths are, and goes through several short
+//     segments or through a part of a long one.  The lengths are read on the
+//     device, so the balance needs nothing from the host.
+//   * A warp takes its own rows of each tile, through a ring of shared-memory
+//     stages of its own that cp.async fills: warps wait for no other until
+//     the segment ends, and loads run ahead over segment borders.  Page
+//     numbers and mask values are fetched one tile ahead of the loads.
+//   * Each warp keeps a running maximum, sum and weighted value sum (online
+//     softmax, fp32).  At the end of a segment the warps' states are joined in
+//     shared memory; a block that has only a part of the segment leaves its
+//     state in the workspace, and the block that arrives last joins the parts
+//     in their order, so the result does not depend on which block it is.
+//
+// Rows that the mask takes out, rows behind the length and rows of bad pages
+// are not loaded: their stage rows are filled with zeros and their score is
+// -inf, so that whatever memory holds there cannot reach the result.
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+
+#include "paged_common.cuh"
+
+namespace gawee {
+namespace kern {
+namespace paged {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxBlocksPerSm = kKvMaxBlocksPerSm;
+constexpr int kMaxSmem = 226 * 1024;  // of a block, beside the kernel's static variables
+constexpr int kMaxDevices = 64;
+
+// --- small pieces -------------------------------------------------------------
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// exp(s - m); a maximum of -inf (nothing attended yet) leaves exp(-inf) = 0, and NaN for a NaN score.
+__device__ __forceinline__ float exp_from(float s, float m) {
+  return exp2_fast((s - (m == -INFINITY ? 0.f : m)) * kLog2e);
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes from global to shared memory; zeros where !valid (src is then not read).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Two fp32 multiply-adds in one instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// --- the two ways to compute a tile ---------------------------------------------
+//
+// Lanes: any types.  L lanes hold a key's row, eight elements each (D <= 8 L),
+// and 32 / L keys are taken at a time.  All products in fp32, two to an
+// instruction.  The partial products of four keys a lane and NH heads are
+// summed over the L lanes by exchanging halves: after it each lane holds
+// complete scores of its own instead of all lanes holding all of them.
+template <class T_, int L, int NH_>
+struct LaneTile {
+  using T = T_;
+  static constexpr int NH = NH_;
+  static constexpr int kKeysAtOnce = 32 / L, kSteps = 4;
+  static constexpr int TK = kSteps * kKeysAtOnce;  // keys of a warp's tile
+  // A stage holds K and V rows of at most TK * 8 L elements: 8 KB in fp32, 4 KB
+  // in 16 bits.  Two blocks of four warps on an SM then have about 128 KB on the way.
+  static constexpr int kStages = sizeof(T) == 4 ? 3 : 6;
+  static constexpr int N = kSteps * NH;                   // scores of a lane before the exchange
+  static constexpr int E = N >= L ? N / L : 1;            // after it
+  static constexpr int kCopies = N >= L ? 1 : L / N;      // lanes that hold the same score
+  static constexpr int HE = E < NH ? E : NH;              // different heads among a lane's scores
+  static constexpr int kScratch = TK * NH + NH;           // floats a warp
+  static constexpr int kVecs = sizeof(T) == 4 ? 2 : 1;    // 16-byte vectors of eight elements
+
+  uint64_t q[NH][4], acc[NH][4];
+  float m[HE], l[HE];
+  int D, lane, l_id, group;
+  bool in0, in1;
+
+  __host__ __device__ static int row_bytes(int D) { return D * (int)sizeof(T); }
+  __device__ static __forceinline__ int chunk_at(int, int chunk) { return chunk; }
+
+  __device__ __forceinline__ int elem(int i) const {  // element of slot i (0 .. 7) of this lane
+    return sizeof(T) == 4 ? (i < 4 ? l_id * 4 + i : (l_id + L) * 4 + i - 4) : l_id * 8 + i;
+  }
+  // First score (step * NH + head) that this lane holds after the exchange.
+  __device__ __forceinline__ int first_score() const { return N >= L ? l_id * E : l_id / kCopies; }
+
+  __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t b, int h0, int nh) {
+    D = p.geom.head_dim;
+    lane = threadIdx.x % 32;
+    l_id = lane % L;
+    group = lane / L;
+    const int vecs = D * (int)sizeof(T) / 16;
+    in0 = l_id < vecs;
+    in1 = l_id + L < vecs;
+#pragma unroll
+    for (int g = 0; g < NH; ++g) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = g < nh && elem(i) < D ? load_act(p.q, p.dt, b * p.q_stride + (int64_t)(h0 + g) * D + elem(i)) * p.scale : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        q[g][i] = pack2(x[2 * i], x[2 * i + 1]);
+        acc[g][i] = 0;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < HE; ++e) {
+      m[e] = -INFINITY;
+      l[e] = 0.f;
+    }
+  }
+
+  __device__ __forceinline__ void load_row(const char* row, uint64_t (&x)[4]) const {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = in0 ? *reinterpret_cast<const float4*>(row + l_id * 16) : make_float4(0, 0, 0, 0);
+      const float4 c = in1 ? *reinterpret_cast<const float4*>(row + (l_id + L) * 16) : make_float4(0, 0, 0, 0);
+      x[0] = pack2(a.x, a.y);
+      x[1] = pack2(a.z, a.w);
+      x[2] = pack2(c.x, c.y);
+      x[3] = pack2(c.z, c.w);
+    } else {
+      const uint4 a = in0 ? *reinterpret_cast<const uint4*>(row + l_id * 16) : make_uint4(0, 0, 0, 0);
+      const T* h = reinterpret_cast<const T*>(&a);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = pack2(to_f(h[2 * i]), to_f(h[2 * i + 1]));
+    }
+  }
+
+  // One tile: K and V rows of TK keys, `add` their mask values; `live` keys
+  // from the first are within the sequence.  Scores go to `scores` (nullptr:
+  // not wanted), [key][group size].
+  __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float* scratch, float* scores,
+                                       int live, int group_size, int nh) {
+    const int rb = row_bytes(D);
+    float s[N];
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      uint64_t x[4];
+      load_row(ks + (st * kKeysAtOnce + group) * rb, x);
+#pragma unroll
+      for (int g = 0; g < NH; ++g) {
+        uint64_t d = mul2(q[g][0], x[0]);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) d = fma2(q[g][i], x[i], d);
+        const float2 f = unpack2(d);
+        s[st * NH + g] = f.x + f.y;
+      }
+    }
+    // sums over the L lanes, halving what a lane holds
+    int cnt = N;
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) {
+      const bool upper = lane & o;
+      if (cnt > 1) {
+        cnt >>= 1;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+          if (i < cnt) {
+            const float send = upper ? s[i] : s[i + cnt], keep = upper ? s[i + cnt] : s[i];
+            s[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+          }
+      } else {
+        s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+      }
+    }
+    const int n0 = first_score();
+    float mx[HE];
+#pragma unroll
+    for (int e = 0; e < HE; ++e) mx[e] = m[e];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int key = (n0 + e) / NH * kKeysAtOnce + group;
+      s[e] += add[key];
+      mx[e % HE] = fmaxf(mx[e % HE], s[e]);
+      if (scores && key < live && (n0 + e) % NH < nh) scores[key * group_size + (n0 + e) % NH] = s[e];
+    }
+    // the maximum over the lanes that hold other keys of the same heads
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      if (o >= L || (o >= kCopies && o * E / kCopies >= NH))
+#pragma unroll
+        for (int e = 0; e < HE; ++e) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
+    bool changed = false;
+#pragma unroll
+    for (int e = 0; e < HE; ++e) changed |= mx[e] != m[e];
+    if (__any_sync(0xffffffffu, changed)) {
+      float* c = scratch + TK * NH;
+#pragma unroll
+      for (int e = 0; e < HE; ++e) {
+        const float f = exp_from(m[e], mx[e]);
+        l[e] *= f;
+        m[e] = mx[e];
+        c[(n0 + e) % NH] = f;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int g = 0; g < NH; ++g) {
+        const uint64_t f = pack2(c[g], c[g]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[g][i] = mul2(acc[g][i], f);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float x = exp_from(s[e], m[e % HE]);
+      l[e % HE] += x;
+      scratch[((n0 + e) / NH * kKeysAtOnce + group) * NH + (n0 + e) % NH] = x;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const int key = st * kKeysAtOnce + group;
+      uint64_t x[4];
+      load_row(vs + key * rb, x);
+#pragma unroll
+      for (int g = 0; g < NH; ++g) {
+        const float f = scratch[key * NH + g];
+        const uint64_t ff = pack2(f, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[g][i] = fma2(ff, x[i], acc[g][i]);
+      }
+    }
+  }
+
+  // The warp's state: ml[2 * head] the maximum, ml[2 * head + 1] the sum, o[head * D + d].
+  __device__ __forceinline__ void dump(float* ml, float* o) {
+    const int n0 = first_score();
+#pragma unroll
+    for (int off = 16; off; off >>= 1)
+      if (off >= L || (off >= kCopies && off * E / kCopies >= NH))
+#pragma unroll
+        for (int e = 0; e < HE; ++e) l[e] += __shfl_xor_sync(0xffffffffu, l[e], off);
+#pragma unroll
+    for (int e = 0; e < HE; ++e) {
+      ml[2 * ((n0 + e) % NH)] = m[e];
+      ml[2 * ((n0 + e) % NH) + 1] = l[e];
+    }
+#pragma unroll
+    for (int g = 0; g < NH; ++g) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2(acc[g][i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+#pragma unroll
+      for (int off = 16; off >= L; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], off);
+      if (group == 0)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (elem(i) < D) o[g * D + elem(i)] = x[i];
+    }
+  }
+};
+
+// Tensor cores: 16-bit pages and activations of one type.  S = Q K^T and O = P V
+// by mma.m16n8k16 with the query heads as rows: the multiplications cost next
+// to nothing beside the loads, where the lanes' fp32 would bound a larger
+// group.  q and K are exact operands.  P is not rounded to the 16-bit type: it
+// is split into two terms (p = hi + lo, relative error 2^-16 in bf16, 2^-21 in
+// fp16).  With up to eight heads hi takes rows 0-7 and lo rows 8-15 of the
+// same product.  D is padded to DT in shared memory; rows are swizzled by 16-byte
+// chunks so that ldmatrix reads eight rows without bank conflicts.
+template <class T_, int DT, int NH_>
+struct MmaTile {
+  using T = T_;
+  static constexpr int NH = NH_;
+  static_assert(NH == 8 || NH == 16, "");
+  static constexpr int TK = DT == 64 ? 32 : 16;
+  static constexpr int kStages = DT == 256 && NH == 16 ? 2 : 3;  // what shared memory holds beside the joint area
+  static constexpr int kScratch = 0;
+  static constexpr int R = NH / 8;  // head rows of a thread
+
+  uint32_t q[DT / 16][2 * R];
+  float acc[DT / 8][4];
+  float m[R], l[R];
+  float scale;
+  int D, lane;
+
+  __host__ __device__ static int row_bytes(int) { return DT * 2; }
+  __device__ static __forceinline__ int chunk_at(int row, int chunk) { return chunk ^ (row & 7); }
+
+  __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t b, int h0, int nh) {
+    D = p.geom.head_dim;
+    lane = threadIdx.x % 32;
+    scale = p.scale;
+    const T* base = static_cast<const T*>(p.q) + b * p.q_stride + (int64_t)h0 * D;
+#pragma unroll
+    for (int k = 0; k < DT / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 2 * R; ++i) {
+        // registers of A: rows g (and g + 8), columns 2c, 2c + 1 (and + 8)
+        const int head = lane / 4 + (R == 2 ? (i & 1) * 8 : 0);
+        const int d = k * 16 + lane % 4 * 2 + (R == 2 ? i >> 1 : i) * 8;
+        T x[2] = {from_f<T>(0.f), from_f<T>(0.f)};
+        if (head < nh && d < D) {  // D is even
+          x[0] = base[(int64_t)head * D + d];
+          x[1] = base[(int64_t)head * D + d + 1];
+        }
+        q[k][i] = *reinterpret_cast<uint32_t*>(x);
+      }
+#pragma unroll
+    for (int j = 0; j < DT / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+    }
+  }
+
+  __device__ static __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    if constexpr (TypeCode<T>::value == DT_BF16)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  __device__ static __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+  }
+  __device__ static __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+  }
+  // Two values as the 16-bit type, and what the rounding left.
+  __device__ static __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    T h[2] = {from_f<T>(x), from_f<T>(y)};
+    T r[2] = {from_f<T>(x - to_f(h[0])), from_f<T>(y - to_f(h[1]))};
+    hi = *reinterpret_cast<uint32_t*>(h);
+    lo = *reinterpret_cast<uint32_t*>(r);
+  }
+
+  __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float*, float* scores, int live,
+                                       int group_size, int nh) {
+    constexpr int RB = DT * 2;
+    const uint32_t kb = smem_u32(ks), vb = smem_u32(vs);
+    float s[TK / 8][4];
+#pragma unroll
+    for (int j = 0; j < TK / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < DT / 16; k += 2)
+#pragma unroll
+      for (int j = 0; j < TK / 8; ++j) {
+        uint32_t r[4];
+        const int row = j * 8 + lane % 8, chunk = 2 * k + lane / 8;
+        ldsm(r, kb + row * RB + chunk_at(row, chunk) * 16);
+        if constexpr (R == 1) {
+          mma(s[j], q[k][0], 0u, q[k][1], 0u, r[0], r[1]);
+          mma(s[j], q[k + 1][0], 0u, q[k + 1][1], 0u, r[2], r[3]);
+        } else {
+          mma(s[j], q[k][0], q[k][1], q[k][2], q[k][3], r[0], r[1]);
+          mma(s[j], q[k + 1][0], q[k + 1][1], q[k + 1][2], q[k + 1][3], r[2], r[3]);
+        }
+      }
+    float mx[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) mx[r] = m[r];
+#pragma unroll
+    for (int j = 0; j < TK / 8; ++j) {
+      const int key = j * 8 + lane % 4 * 2;
+      const float2 a = *reinterpret_cast<const float2*>(add + key);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        s[j][2 * r] = fmaf(s[j][2 * r], scale, a.x);
+        s[j][2 * r + 1] = fmaf(s[j][2 * r + 1], scale, a.y);
+        mx[r] = fmaxf(mx[r], fmaxf(s[j][2 * r], s[j][2 * r + 1]));
+        const int head = lane / 4 + 8 * r;
+        if (scores && head < nh) {
+          if (key < live) scores[key * group_size + head] = s[j][2 * r];
+          if (key + 1 < live) scores[(key + 1) * group_size + head] = s[j][2 * r + 1];
+        }
+      }
+    }
+    bool changed = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+      changed |= mx[r] != m[r];
+    }
+    if (__any_sync(0xffffffffu, changed)) {
+      float c[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        c[r] = exp_from(m[r], mx[r]);
+        l[r] *= c[r];
+        m[r] = mx[r];
+      }
+#pragma unroll
+      for (int j = 0; j < DT / 8; ++j) {
+        acc[j][0] *= c[0];
+        acc[j][1] *= c[0];
+        acc[j][2] *= c[R - 1];
+        acc[j][3] *= c[R - 1];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < TK / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 2 * R; ++i) {
+        s[j][i] = exp_from(s[j][i], m[i / 2]);
+        l[i / 2] += s[j][i];
+      }
+#pragma unroll
+    for (int kk = 0; kk < TK / 16; ++kk) {
+      uint32_t hi[2][R], lo[2][R];  // [columns 0-7 / 8-15 of the 16 keys][head rows]
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int r = 0; r < R; ++r) split(s[2 * kk + c][2 * r], s[2 * kk + c][2 * r + 1], hi[c][r], lo[c][r]);
+#pragma unroll
+      for (int j = 0; j < DT / 8; j += 2) {
+        uint32_t r[4];
+        const int row = kk * 16 + lane / 8 % 2 * 8 + lane % 8, chunk = j + lane / 16;
+        ldsm_t(r, vb + row * RB + chunk_at(row, chunk) * 16);
+        if constexpr (R == 1) {
+          mma(acc[j], hi[0][0], lo[0][0], hi[1][0], lo[1][0], r[0], r[1]);
+          mma(acc[j + 1], hi[0][0], lo[0][0], hi[1][0], lo[1][0], r[2], r[3]);
+        } else {
+          mma(acc[j], hi[0][0], hi[0][1], hi[1][0], hi[1][1], r[0], r[1]);
+          mma(acc[j], lo[0][0], lo[0][1], lo[1][0], lo[1][1], r[0], r[1]);
+          mma(acc[j + 1], hi[0][0], hi[0][1], hi[1][0], hi[1][1], r[2], r[3]);
+          mma(acc[j + 1], lo[0][0], lo[0][1], lo[1][0], lo[1][1], r[2], r[3]);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void dump(float* ml, float* o) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      const int head = lane / 4 + 8 * r;
+      ml[2 * head] = m[r];
+      ml[2 * head + 1] = l[r];
+#pragma unroll
+      for (int j = 0; j < DT / 8; ++j) {
+        const int d = j * 8 + lane % 4 * 2;
+        if (d < D) {
+          o[head * D + d] = R == 1 ? acc[j][0] + acc[j][2] : acc[j][2 * r];
+          o[head * D + d + 1] = R == 1 ? acc[j][1] + acc[j][3] : acc[j][2 * r + 1];
+        }
+      }
+    }
+  }
+};
+
+// --- the kernel -------------------------------------------------------------------
+
+// Where a block is in its run of tiles.
+struct Cursor {
+  int b = 0, kvh = 0, chunk = 0, tile = 0, tiles = 0;
+  int len = 0;
+};
+
+// Rows that take part: 0 for a length beyond the limit, -1 for no sequence.
+__device__ __forceinline__ int length_of(const KvAttendParams& p, int b) {
+  const int n = p.lengths[b];
+  return n < 0 ? -1 : n > p.max_len ? 0 : n;
+}
+template <int TILE>
+__device__ __forceinline__ int tiles_of(int len) {  // an empty sequence takes one, for its zeros
+  return len < 0 ? 0 : len == 0 ? 1 : (len + TILE - 1) / TILE;
+}
+
+// Shared memory in bytes: the warps' stages, their mask values, scratch and the states that are joined.
+template <class P>
+__host__ __device__ constexpr int attend_stage_bytes(int row_bytes) { return 2 * P::TK * row_bytes; }
+template <class P>
+inline int attend_smem(int row_bytes, int D) {
+  return kWarps * (P::kStages * (attend_stage_bytes<P>(row_bytes) + P::TK * 4) + P::kScratch * 4) +
+         kWarps * P::NH * (D + 2) * 4;
+}
+
+template <class P>
+__global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_constant__ KvAttendParams p) {
+  using T = typename P::T;
+  constexpr int TK = P::TK, TILE = kWarps * TK, NS = P::kStages, NH = P::NH;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ long long s_warp[kWarps], s_base;
+  __shared__ int s_b0, s_last;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int D = p.geom.head_dim, kv = p.geom.kv_heads, group = p.heads / kv, chunks = (group + NH - 1) / NH;
+  const int per_tile = kv * chunks;  // segments of a sequence
+
+  // The block's run of tiles: prefix sums of the sequences' tiles, each thread a slice of the batch.
+  long long t0, t1, total, blocks;
+  {
+    const int slice = (p.batch + kThreads - 1) / kThreads, b0 = min(tid * slice, p.batch), b1 = min(b0 + slice, p.batch);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += tiles_of<TILE>(length_of(p, b));
+    long long scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += up;
+    }
+    if (lane == 31) s_warp[warp] = scan;
+    __syncthreads();
+    long long before = 0, sum = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) before = sum;
+      sum += s_warp[w];
+    }
+    total = sum * per_tile;
+    blocks = min((long long)gridDim.x, total);  // every one of them has a tile
+    if (blockIdx.x >= blocks) return;
+    t0 = total * blockIdx.x / blocks;
+    t1 = total * (blockIdx.x + 1) / blocks;
+    before = (before + scan - mine) * per_tile;
+    if (t0 >= before && t0 < before + mine * per_tile) {  // this thread's slice holds the first tile
+      int b = b0;
+      for (;; ++b) {
+        const long long n = (long long)tiles_of<TILE>(length_of(p, b)) * per_tile;
+        if (t0 < before + n) break;
+        before += n;
+      }
+      s_b0 = b;
+      s_base = before;
+    }
+    __syncthreads();
+  }
+
+  auto enter = [&](Cursor& c) {  // at the first tile of sequence c.b, or of the next one that has tiles
+    for (;;) {
+      c.len = length_of(p, c.b);
+      c.tiles = tiles_of<TILE>(c.len);
+      if (c.tiles) return;
+      ++c.b;
+    }
+  };
+  auto advance = [&](Cursor& c) {
+    if (++c.tile < c.tiles) return;
+    c.tile = 0;
+    if (++c.chunk < chunks) return;
+    c.chunk = 0;
+    if (++c.kvh < kv) return;
+    c.kvh = 0;
+    ++c.b;
+    enter(c);
+  };
+  Cursor use;
+  use.b = s_b0;
+  use.len = length_of(p, use.b);
+  use.tiles = tiles_of<TILE>(use.len);
+  {
+    const long long in = t0 - s_base;  // tiles into the sequence: (kvh, chunk, tile)
+    use.tile = (int)(in % use.tiles);
+    const int seg = (int)(in / use.tiles);
+    use.chunk = seg % chunks;
+    use.kvh = seg / chunks;
+  }
+  Cursor load = use;
+  const int count = (int)(t1 - t0);
+
+  // the warp's part of shared memory
+  const int rb = P::row_bytes(D), stage_bytes = attend_stage_bytes<P>(rb);
+  char* ring = smem + warp * NS * stage_bytes;
+  float* adds = reinterpret_cast<float*>(smem + kWarps * NS * stage_bytes) + warp * NS * TK;
+  float* scratch = reinterpret_cast<float*>(smem + kWarps * NS * (stage_bytes + TK * 4)) + warp * P::kScratch;
+  float* joint = reinterpret_cast<float*>(smem + kWarps * (NS * (stage_bytes + TK * 4) + P::kScratch * 4));
+  if constexpr (P::kScratch == 0) {  // tensor cores read the padding of K up to DT: zeros, never written again
+    if (rb != D * (int)sizeof(T)) {
+      for (int i = lane; i < NS * stage_bytes / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+    }
+  }
+
+  // Fetching a tile: lane r holds the page and the mask value of the warp's row r.
+  int f_page = -1;
+  float f_add = 0.f;
+  auto fetch = [&](const Cursor& c) {
+    const int i = c.tile * TILE + warp * TK + lane;
+    f_page = -1;
+    f_add = -INFINITY;
+    if (lane < TK && i < c.len) {
+      const int col = i / p.geom.page_size;
+      f_page = col < p.table_cols ? p.table[c.b * p.table_stride + col] : -1;
+      f_add = p.mask ? p.mask[c.b * p.mask_stride + i] : 0.f;
+    }
+  };
+  // lane's first vector among a tile's rows, and the step to its next one
+  const int vecs = D * (int)sizeof(T) / 16;
+  const int row_step = 32 / vecs, col_step = 32 % vecs, row_0 = lane / vecs, col_0 = lane % vecs;
+  auto issue = [&](const Cursor& c, int stage) {
+    const int first = c.tile * TILE + warp * TK, i = first + lane;
+    char* ks = ring + stage * stage_bytes;
+    if (first < c.len) {
+      char* vs = ks + TK * rb;
+      long long off = -1;
+      bool fresh = false;
+      if (lane < TK && i < c.len) {
+        if (f_page < 0 || f_page >= p.geom.num_pages) {
+          set_status(p.status, ST_KV_PAGE);
+          f_add = -INFINITY;
+        } else {
+          off = row_offset(f_page, c.kvh, i % p.geom.page_size, p.geom) * (long long)sizeof(T);
+          fresh = p.k && i == c.len - 1;
+        }
+      }
+      if (lane < TK) adds[stage * TK + lane] = f_add;
+      const unsigned fresh_row = __ballot_sync(0xffffffffu, fresh);
+      const long long fresh_off = __shfl_sync(0xffffffffu, off, fresh_row ? __ffs(fresh_row) - 1 : 0);
+      if (f_add == -INFINITY || fresh) off = -1;  // nothing to load
+      // the new token's row is written below, unless the mask takes it out
+      const int new_row = fresh_row ? __ffs(fresh_row) - 1 : 0;
+      const bool put_new = fresh_row && __shfl_sync(0xffffffffu, f_add, new_row) != -INFINITY;
+      int row = row_0, col = col_0;
+      for (int v = 0; v < TK * vecs; v += 32) {
+        const long long o = __shfl_sync(0xffffffffu, off, row & 31);
+        if (row < TK && !(put_new && row == new_row)) {
+          const bool ok = o >= 0;
+          const long long at = ok ? o + col * 16 : 0;
+          const int s = row * rb + P::chunk_at(row, col) * 16;
+          copy16(smem_u32(ks + s), static_cast<const char*>(p.k_pages) + at, ok);
+          copy16(smem_u32(vs + s), static_cast<const char*>(p.v_pages) + at, ok);
+        }
+        row += row_step;
+        col += col_step;
+        if (col >= vecs) {
+          col -= vecs;
+          ++row;
+        }
+      }
+      if (fresh_row) {
+        // the new token's row comes from the call's arguments, rounded as it is
+        // stored; the block of the first chunk of heads stores it
+        for (int d = lane; d < D; d += 32) {
+          const T k = from_f<T>(load_act(p.k, p.dt, c.b * p.k_stride + c.kvh * D + d));
+          const T v = from_f<T>(load_act(p.v, p.dt, c.b * p.v_stride + c.kvh * D + d));
+          if (put_new) {
+            const int s = new_row * rb + P::chunk_at(new_row, d * (int)sizeof(T) / 16) * 16 + d * (int)sizeof(T) % 16;
+            *reinterpret_cast<T*>(ks + s) = k;
+            *reinterpret_cast<T*>(vs + s) = v;
+          }
+          if (c.chunk == 0) {
+            reinterpret_cast<T*>(static_cast<char*>(p.k_pages) + fresh_off)[d] = k;
+            reinterpret_cast<T*>(static_cast<char*>(p.v_pages) + fresh_off)[d] = v;
+          }
+        }
+      }
+    }
+  };
+
+  // fill the ring
+  int issued = 0;
+  fetch(load);
+#pragma unroll 1
+  for (; issued < NS - 1; ++issued) {
+    if (issued < count) {
+      issue(load, issued);
+      if (issued + 1 < count) {
+        advance(load);
+        fetch(load);
+      }
+    }
+    copy_commit();
+  }
+
+  P state;
+  bool fresh_segment = true;
+  long long seg_begin = t0 - use.tile;  // the segment's first tile
+#pragma unroll 1
+  for (int j = 0; j < count; ++j) {
+    const int h0 = use.kvh * group + use.chunk * NH, nh = min(NH, group - use.chunk * NH);
+    if (fresh_segment) state.begin(p, use.b, h0, nh);
+    fresh_segment = false;
+    copy_wait<NS - 2>();
+    __syncwarp();
+    if (issued < count) {
+      issue(load, issued % NS);
+      if (++issued < count) {
+        advance(load);
+        fetch(load);
+      }
+    }
+    copy_commit();
+    const int first = use.tile * TILE + warp * TK;
+    if (first < use.len) {
+      const int stage = j % NS;
+      float* scores = p.weights_out
+                          ? p.scores + (((long long)use.b * kv + use.kvh) * p.max_len + first) * group + use.chunk * NH
+                          : nullptr;
+      state.tile(ring + stage * stage_bytes, ring + stage * stage_bytes + TK * rb, adds + stage * TK, scratch, scores,
+                 use.len - first, group, nh);
+    }
+    const bool seg_end = use.tile + 1 == use.tiles;
+    if (seg_end || j + 1 == count) {
+      // join the warps
+      float* ml = joint;                   // [warp][NH][2]
+      float* o = joint + kWarps * NH * 2;  // [warp][NH][D]
+      state.dump(ml + warp * NH * 2, o + warp * NH * D);
+      __syncthreads();
+      const long long seg_last = seg_begin + use.tiles - 1;
+      const bool whole = seg_begin >= t0 && seg_end;
+      const int slot = seg_begin <= t0 ? 0 : 1;
+      float* part = p.parts + (2ll * blockIdx.x + slot) * NH * (D + 2);
+      for (int x = tid; x < nh * D; x += kThreads) {
+        const int h = x / D, d = x % D;
+        float mt = -INFINITY, lt = 0.f, ot = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, ml[(w * NH + h) * 2]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float c = exp_from(ml[(w * NH + h) * 2], mt);
+          lt += ml[(w * NH + h) * 2 + 1] * c;
+          ot += o[(w * NH + h) * D + d] * c;
+        }
+        if (whole) {
+          store_act(p.out, p.dt, use.b * p.out_stride + (int64_t)(h0 + h) * D + d, lt != 0.f ? ot / lt : 0.f);
+          if (p.weights_out && d == 0) {
+            p.stats[((int64_t)use.b * p.heads + h0 + h) * 2] = mt;
+            p.stats[((int64_t)use.b * p.heads + h0 + h) * 2 + 1] = lt;
+          }
+        } else {
+          part[2 * NH + x] = ot;
+          if (d == 0) {
+            part[2 * h] = mt;
+            part[2 * h + 1] = lt;
+          }
+        }
+      }
+      if (!whole) {
+        // block that holds tile t: the largest i with floor(total * i / blocks) <= t
+        const int c0 = (int)(((seg_begin + 1) * blocks - 1) / total);
+        const int c1 = (int)(((seg_last + 1) * blocks - 1) / total);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          // wraps to 0 with the last arrival: ready for the next call
+          const unsigned old = atomicInc(p.arrived + ((int64_t)use.b * kv + use.kvh) * chunks + use.chunk, c1 - c0);
+          s_last = old == (unsigned)(c1 - c0);
+        }
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          const bool c0_first = total * c0 / blocks >= seg_begin;  // the segment is the first of block c0's run
+          auto part_of = [&](int c) { return p.parts + (2ll * c + (c == c0 && !c0_first ? 1 : 0)) * NH * (D + 2); };
+          for (int x = tid; x < nh * D; x += kThreads) {
+            const int h = x / D, d = x % D;
+            float mt = -INFINITY, lt = 0.f, ot = 0.f;
+            for (int c = c0; c <= c1; ++c) mt = fmaxf(mt, __ldcg(part_of(c) + 2 * h));
+            for (int c = c0; c <= c1; ++c) {
+              const float* q = part_of(c);
+              const float f = exp_from(__ldcg(q + 2 * h), mt);
+              lt += __ldcg(q + 2 * h + 1) * f;
+              ot += __ldcg(q + 2 * NH + x) * f;
+            }
+            store_act(p.out, p.dt, use.b * p.out_stride + (int64_t)(h0 + h) * D + d, lt != 0.f ? ot / lt : 0.f);
+            if (p.weights_out && d == 0) {
+              p.stats[((int64_t)use.b * p.heads + h0 + h) * 2] = mt;
+              p.stats[((int64_t)use.b * p.heads + h0 + h) * 2 + 1] = lt;
+            }
+          }
+        }
+      }
+      __syncthreads();  // the joint area is free again
+      if (j + 1 < count) seg_begin = seg_last + 1;
+      fresh_segment = true;
+    }
+    if (j + 1 < count) advance(use);
+  }
+  copy_wait<0>();
+  if (blockIdx.x == 0)  // lengths that length_of took as 0
+    for (int b = tid; b < p.batch; b += kThreads)
+      if (p.lengths[b] > p.max_len) set_status(p.status, ST_KV_LENGTH);
+}
+
+// Blocks of this kernel that an SM holds, at most kMaxBlocksPerSm; asked once
+// per device and shared-memory size.
+template <class P>
+cudaError_t blocks_per_sm(int device, int smem, int* out) {
+  static std::atomic<int64_t> known[kMaxDevices];  // smem << 8 | blocks
+  if (device < kMaxDevices) {
+    const int64_t k = known[device].load(std::memory_order_relaxed);
+    if (k >> 8 == smem && k) {
+      *out = (int)(k & 255);
+      return cudaSuccess;
+    }
+  }
+  // the limit covers every head dim, so that calls of two threads do not undo each other's
+  cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  int n = 0;
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attend_kernel<P>, kThreads, smem);
+  if (e != cudaSuccess) return e;
+  *out = std::min(std::max(n, 1), kMaxBlocksPerSm);
+  if (device < kMaxDevices) known[device].store((int64_t)smem << 8 | *out, std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
+template <class P>
+cudaError_t attend_launch(const KvAttendParams& p, cudaStream_t s) {
+  const int D = p.geom.head_dim, smem = attend_smem<P>(P::row_bytes(D), D);
+  int per_sm = 0;
+  if (cudaError_t e = blocks_per_sm<P>(p.device, smem, &per_sm)) return e;
+  kv_attend_kernel<P><<<p.sms * per_sm, kThreads, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+// The lanes' kernel for this head dim and group.
+template <class T, int L>
+cudaError_t attend_lanes_l(const KvAttendParams& p, cudaStream_t s) {
+  const int group = p.heads / p.geom.kv_heads;
+  if (group <= 1) return attend_launch<LaneTile<T, L, 1>>(p, s);
+  if (group <= 2) return attend_launch<LaneTile<T, L, 2>>(p, s);
+  if (group <= 4) return attend_launch<LaneTile<T, L, 4>>(p, s);
+  return attend_launch<LaneTile<T, L, 8>>(p, s);
+}
+template <class T>
+cudaError_t attend_lanes(const KvAttendParams& p, cudaStream_t s) {
+  const int D = p.geom.head_dim;
+  if (D <= 32) return attend_lanes_l<T, 4>(p, s);
+  if (D <= 64) return attend_lanes_l<T, 8>(p, s);
+  if (D <= 128) return attend_lanes_l<T, 16>(p, s);
+  return attend_lanes_l<T, 32>(p, s);
+}
+template <class T, int NH>
+cudaError_t attend_mma(const KvAttendParams& p, cudaStream_t s) {
+  const int D = p.geom.head_dim;
+  if (D <= 64) return attend_launch<MmaTile<T, 64, NH>>(p, s);
+  if (D <= 128) return attend_launch<MmaTile<T, 128, NH>>(p, s);
+  return attend_launch<MmaTile<T, 256, NH>>(p, s);
+}
+template <class T>
+cudaError_t attend_16bit(const KvAttendParams& p, cudaStream_t s) {
+  const int group = p.heads / p.geom.kv_heads;
+  if (p.dt == TypeCode<T>::value && group > 1)
+    return group <= 8 ? attend_mma<T, 8>(p, s) : attend_mma<T, 16>(p, s);
+  return attend_lanes<T>(p, s);
+}
+
+}  // namespace paged
+}  // namespace kern
+}  // namespace gawee

@@ -1,0 +1,10 @@
+// Attention over a paged key/value cache of f16 pages.
+#include "paged_attend.cuh"
+
+namespace gawee {
+namespace kern {
+
+cudaError_t launch_kv_attend_f16(const KvAttendParams& p, cudaStream_t s) { return paged::attend_16bit<__half>(p, s); }
+
+}  // namespace kern
+}  // namespace gawee

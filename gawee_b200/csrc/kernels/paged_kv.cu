@@ -1,69 +1,17 @@
-// Kernels of the paged key/value cache: append, attention of one new token
-// over the pages, and eviction by accumulated attention weight.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+// Kernels of the paged key/value cache: append, the weights' pass of
+// attend (the attention itself is in paged_attend.cuh) and eviction by
+// accumulated attention weight.
 #include <algorithm>
 #include <cstdint>
 
-#include "paged_kv.h"
+#include "paged_common.cuh"
 
 namespace gawee {
 namespace kern {
 
+using namespace paged;
+
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ void set_status(int* st, int code) {
-  if (st) atomicCAS(st, 0, code);
-}
-
-// --- element types ----------------------------------------------------------
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <class T>
-__device__ __forceinline__ T from_f(float x);
-template <>
-__device__ __forceinline__ float from_f<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
-// Element i of an activation array whose type is only known at run time: the
-// few values a block reads once or writes once.
-__device__ __forceinline__ float load_act(const void* p, int dt, int64_t i) {
-  if (dt == DT_F32) return static_cast<const float*>(p)[i];
-  if (dt == DT_F16) return to_f(static_cast<const __half*>(p)[i]);
-  return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-__device__ __forceinline__ void store_act(void* p, int dt, int64_t i, float x) {
-  if (dt == DT_F32) static_cast<float*>(p)[i] = x;
-  else if (dt == DT_F16) static_cast<__half*>(p)[i] = from_f<__half>(x);
-  else static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(x);
-}
-
-// Eight consecutive values of a 16-byte aligned row.
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const T* h = reinterpret_cast<const T*>(&a);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f(h[i]);
-}
-
-__device__ __forceinline__ float warp_sum(float x) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
-}
 
 // --- append -------------------------------------------------------------------
 // One thread per element of a token's row over the heads.
@@ -72,8 +20,7 @@ __global__ void kv_append_kernel(KvAppendParams p) {
   const int row = p.geom.kv_heads * p.geom.head_dim;
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     const int64_t seq = p.sequences ? (int64_t)p.sequences[t] : t;
-    int64_t pos = p.positions[t];
-    if (p.last) pos = pos > p.last ? -1 : pos - 1;
+    const int64_t pos = p.positions[t];
     if (seq < 0 || pos < 0) continue;
     const int64_t page = seq < p.batch ? page_of(p.table + seq * p.table_stride, p.table_cols, pos, p.geom) : -1;
     if (page < 0) {
@@ -90,103 +37,6 @@ __global__ void kv_append_kernel(KvAppendParams p) {
   }
 }
 
-// --- attend --------------------------------------------------------------------
-// One block per (sequence, key/value head, chunk of query heads).  A warp takes
-// every fourth key; lane l holds elements 8l .. 8l+7 of the row.
-constexpr int kAttendThreads = 128;
-
-template <class T>
-__global__ void __launch_bounds__(kAttendThreads) kv_attend_kernel(KvAttendParams p) {
-  constexpr int kWarps = kAttendThreads / 32;
-  const int D = p.geom.head_dim, group = p.heads / p.geom.kv_heads;
-  const int chunks = (group + kKvHeadChunk - 1) / kKvHeadChunk;
-  const int chunk = blockIdx.x % chunks, kvh = blockIdx.x / chunks % p.geom.kv_heads;
-  const int b = blockIdx.x / chunks / p.geom.kv_heads;
-  const int h0 = kvh * group + chunk * kKvHeadChunk, nh = min(kKvHeadChunk, group - chunk * kKvHeadChunk);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const bool active = lane * 8 < D;
-  int64_t len = p.lengths[b];
-  if (len < 0) return;
-  if (len > p.max_len) {
-    if (threadIdx.x == 0) set_status(p.status, ST_KV_LENGTH);
-    len = 0;
-  }
-  float q[kKvHeadChunk][8], acc[kKvHeadChunk][8], m[kKvHeadChunk], l[kKvHeadChunk];
-#pragma unroll
-  for (int g = 0; g < kKvHeadChunk; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      acc[g][i] = 0.f;
-      q[g][i] = active && g < nh ? load_act(p.q, p.dt, b * p.q_stride + (int64_t)(h0 + g) * D + lane * 8 + i) * p.scale
-                                 : 0.f;
-    }
-  }
-  const int32_t* table = p.table + b * p.table_stride;
-  for (int64_t i = warp; i < len; i += kWarps) {
-    const int64_t page = page_of(table, p.table_cols, i, p.geom);
-    const float add = p.mask ? p.mask[b * p.mask_stride + i] : 0.f;
-    if (page < 0 && lane == 0) set_status(p.status, ST_KV_PAGE);
-    const bool out = page < 0 || add == -INFINITY;  // takes no part, whatever its rows hold
-    float x[8] = {};
-    const int64_t o = out ? 0 : row_offset(page, kvh, (int)(i % p.geom.page_size), p.geom) + lane * 8;
-    if (active && !out) load8(static_cast<const T*>(p.k_pages) + o, x);
-    float s[kKvHeadChunk];
-#pragma unroll
-    for (int g = 0; g < kKvHeadChunk; ++g) {
-      float d = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d = fmaf(q[g][j], x[j], d);
-      s[g] = out ? -INFINITY : warp_sum(d) + add;
-    }
-    if (p.weights_out && lane == 0)
-      for (int g = 0; g < nh; ++g) p.scores[((int64_t)b * p.heads + h0 + g) * p.max_len + i] = s[g];
-    if (out) continue;
-    if (active) load8(static_cast<const T*>(p.v_pages) + o, x);
-#pragma unroll
-    for (int g = 0; g < kKvHeadChunk; ++g) {
-      const float mn = fmaxf(m[g], s[g]);
-      const float c = mn == -INFINITY ? 1.f : exp2f((m[g] - mn) * kLog2e);
-      const float e = mn == -INFINITY ? 0.f : exp2f((s[g] - mn) * kLog2e);
-      m[g] = mn;
-      l[g] = l[g] * c + e;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[g][j] = fmaf(e, x[j], acc[g][j] * c);
-    }
-  }
-  // join the warps
-  __shared__ float sm[kWarps][kKvHeadChunk], sl[kWarps][kKvHeadChunk], so[kWarps][256];
-#pragma unroll
-  for (int g = 0; g < kKvHeadChunk; ++g)
-    if (lane == 0) {
-      sm[warp][g] = m[g];
-      sl[warp][g] = l[g];
-    }
-  __syncthreads();
-  for (int g = 0; g < nh; ++g) {
-    float mt = -INFINITY, lt = 0.f;
-    for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, sm[w][g]);
-    for (int w = 0; w < kWarps; ++w) lt += sm[w][g] == -INFINITY ? 0.f : sl[w][g] * exp2f((sm[w][g] - mt) * kLog2e);
-#pragma unroll
-    for (int gg = 0; gg < kKvHeadChunk; ++gg)
-      if (gg == g && active)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) so[warp][lane * 8 + j] = acc[gg][j];
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += kAttendThreads) {
-      float o = 0.f;
-      for (int w = 0; w < kWarps; ++w) o += sm[w][g] == -INFINITY ? 0.f : so[w][d] * exp2f((sm[w][g] - mt) * kLog2e);
-      store_act(p.out, p.dt, b * p.out_stride + (int64_t)(h0 + g) * D + d, lt != 0.f ? o / lt : 0.f);
-    }
-    if (p.weights_out && threadIdx.x == 0) {
-      p.stats[((int64_t)b * p.heads + h0 + g) * 2] = mt;
-      p.stats[((int64_t)b * p.heads + h0 + g) * 2 + 1] = lt;
-    }
-    __syncthreads();
-  }
-}
-
 // weights_out = weights + the attention weights of this step, summed over the
 // query heads of the key/value head in their order.
 __global__ void kv_weights_kernel(KvAttendParams p) {
@@ -194,12 +44,13 @@ __global__ void kv_weights_kernel(KvAttendParams p) {
   const int group = p.heads / p.geom.kv_heads;
   const int64_t len = p.lengths[b];
   if (len > p.max_len) return;
+  const float* stats = p.stats + ((int64_t)b * p.heads + kvh * group) * 2;
   for (int64_t i = (int64_t)blockIdx.y * blockDim.x + threadIdx.x; i < len; i += (int64_t)gridDim.y * blockDim.x) {
+    const float* s = p.scores + ((int64_t)blockIdx.x * p.max_len + i) * group;
     float w = 0.f;
     for (int g = 0; g < group; ++g) {
-      const int64_t row = (int64_t)b * p.heads + kvh * group + g;
-      const float s = p.scores[row * p.max_len + i], m = p.stats[row * 2], l = p.stats[row * 2 + 1];
-      w += s == -INFINITY ? 0.f : exp2f((s - m) * kLog2e) / l;
+      const float m = stats[2 * g], l = stats[2 * g + 1];
+      w += s[g] == -INFINITY ? 0.f : exp2f((s[g] - m) * kLog2e) / l;
     }
     const float before = p.weights ? p.weights[b * p.w_batch + kvh * p.w_stride + i] : 0.f;
     p.weights_out[b * p.wo_batch + kvh * p.wo_stride + i] = before + w;
@@ -365,31 +216,9 @@ cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t s) {
 
 cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s) {
   if (p.batch == 0) return cudaSuccess;
-  if (p.k) {
-    // the new token of sequence b is its last row
-    KvAppendParams a{};
-    a.geom = p.geom;
-    a.k_pages = p.k_pages;
-    a.v_pages = p.v_pages;
-    a.page_dt = p.page_dt;
-    a.k = p.k;
-    a.v = p.v;
-    a.dt = p.dt;
-    a.k_stride = p.k_stride;
-    a.v_stride = p.v_stride;
-    a.tokens = p.batch;
-    a.positions = p.lengths;
-    a.table = p.table;
-    a.table_stride = p.table_stride;
-    a.table_cols = p.table_cols;
-    a.batch = p.batch;
-    a.last = p.max_len;
-    a.status = p.status;
-    if (cudaError_t e = launch_kv_append(a, s)) return e;
-  }
-  const int group = p.heads / p.geom.kv_heads, chunks = (group + kKvHeadChunk - 1) / kKvHeadChunk;
-  const unsigned grid = (unsigned)(p.batch * p.geom.kv_heads * chunks);
-  cudaError_t e = by_type(p.page_dt, [&](auto t) { kv_attend_kernel<decltype(t)><<<grid, kAttendThreads, 0, s>>>(p); });
+  cudaError_t e = p.page_dt == DT_F32   ? launch_kv_attend_f32(p, s)
+                  : p.page_dt == DT_F16 ? launch_kv_attend_f16(p, s)
+                                        : launch_kv_attend_bf16(p, s);
   if (e == cudaSuccess && p.weights_out) {
     kv_weights_kernel<<<dim3((unsigned)(p.batch * p.geom.kv_heads), 16), 256, 0, s>>>(p);
     e = cudaGetLastError();

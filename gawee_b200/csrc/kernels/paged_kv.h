@@ -10,9 +10,10 @@
 namespace gawee {
 namespace kern {
 
-// Query heads of one key/value head that a block computes together; a larger
-// group takes several blocks, which read the same keys.
-constexpr int kKvHeadChunk = 8;
+// Attention: query heads of a key/value head that a block computes together at
+// most (a larger group takes several runs over the same keys) and at least, and
+// the blocks that an SM holds at most.  They size the workspace.
+constexpr int kKvHeadsMost = 16, kKvHeadsLeast = 8, kKvMaxBlocksPerSm = 4;
 
 // Rows of new tokens into the pages: token t's key k[t * k_stride + h * D ..]
 // goes to row positions[t] of sequence sequences[t] (nullptr: sequence t).  A
@@ -29,7 +30,6 @@ struct KvAppendParams {
   const int32_t* table;
   int64_t table_stride, table_cols;
   int batch;
-  int64_t last;  // nonzero: positions are lengths, the row is the last one; a length above `last` stores nothing
   int* status;
 };
 cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t s);
@@ -56,11 +56,18 @@ struct KvAttendParams {
   const float* weights;  // accumulators before (nullptr with weights_out set: zeros) ..
   float* weights_out;    // .. and after this step (nullptr: not wanted)
   int64_t w_stride, w_batch, wo_stride, wo_batch;
-  float* scores;         // [batch][heads][max_len], with weights_out
+  float* scores;         // [batch][kv_heads][max_len][heads / kv_heads], with weights_out
   float* stats;          // [batch][heads][2]: maximum and sum, with weights_out
+  float* parts;          // states of parts of segments: two a block, heads of a block * (D + 2) each
+  unsigned* arrived;     // [batch][kv_heads][chunks of heads] parts that are there; 0 between calls
+  int device, sms;
   int* status;
 };
 cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s);
+// The same for pages of one type (paged_attend_*.cu), without the weights' pass.
+cudaError_t launch_kv_attend_f32(const KvAttendParams& p, cudaStream_t s);
+cudaError_t launch_kv_attend_f16(const KvAttendParams& p, cudaStream_t s);
+cudaError_t launch_kv_attend_bf16(const KvAttendParams& p, cudaStream_t s);
 
 // Eviction by accumulated weight.
 struct KvEvictParams {
