@@ -37,7 +37,6 @@ struct gawee_kv {
 
 namespace {
 
-using gawee::kern::kKvHeadsLeast;
 using gawee::kern::kKvHeadsMost;
 using gawee::kern::kKvMaxBlocksPerSm;
 using gawee::kern::PageGeom;
@@ -169,13 +168,12 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     if (e == cudaSuccess && d.weights) e = cudaMalloc((void**)&kv->stats, sizeof(float) * 2 * rows);
     if (e == cudaSuccess && d.weights)
       e = cudaMalloc((void**)&kv->scores, sizeof(float) * rows * d.max_pages * d.page_size);
-    const int group = d.heads / d.kv_heads, block_heads = group > kKvHeadsLeast ? kKvHeadsMost : kKvHeadsLeast;
-    const size_t counters = (size_t)d.max_batch * d.kv_heads * ((group + kKvHeadsLeast - 1) / kKvHeadsLeast);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess)
-      e = cudaMalloc((void**)&kv->parts, sizeof(float) * 2 * kv->sms * kKvMaxBlocksPerSm * block_heads * (d.head_dim + 2));
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->arrived, sizeof(unsigned) * counters);
-    if (e == cudaSuccess) e = cudaMemset(kv->arrived, 0, sizeof(unsigned) * counters);
+    const size_t parts = (size_t)2 * kv->sms * kKvMaxBlocksPerSm;
+    const int block_heads = d.heads / d.kv_heads > 8 ? kKvHeadsMost : 8;
+    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->parts, sizeof(float) * parts * block_heads * (d.head_dim + 2));
+    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->arrived, sizeof(unsigned) * 2 * parts);
+    if (e == cudaSuccess) e = cudaMemset(kv->arrived, 0, sizeof(unsigned) * 2 * parts);
     if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
@@ -315,6 +313,9 @@ gawee_status gawee_kv_attend(gawee_kv* kv, const gawee_kv_attend_args* a, void* 
     p.arrived = kv->arrived;
     p.device = kv->device;
     p.sms = kv->sms;
+    p.page_shift = -1;
+    for (int b = 0; b <= 16; ++b)
+      if (kv->geom.page_size == 1 << b) p.page_shift = b;
     p.status = kv->status;
     return run_on(kv, kName, [&] { return launch_kv_attend(p, static_cast<cudaStream_t>(stream)); });
   });

@@ -39,7 +39,7 @@ namespace paged {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBlocksPerSm = kKvMaxBlocksPerSm;
-constexpr int kMaxSmem = 226 * 1024;  // of a block, beside the kernel's static variables
+constexpr int kMaxSmem = 220 * 1024;  // of a block, beside the kernel's static variables
 constexpr int kMaxDevices = 64;
 
 // --- small pieces -------------------------------------------------------------
@@ -59,6 +59,9 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -93,7 +96,8 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // instruction.  The partial products of four keys a lane and NH heads are
 // summed over the L lanes by exchanging halves: after it each lane holds
 // complete scores of its own instead of all lanes holding all of them.
-template <class T_, int L, int NH_>
+// With FULL, D is 8 L: known to the compiler, no lane idle.
+template <class T_, int L, int NH_, bool FULL>
 struct LaneTile {
   using T = T_;
   static constexpr int NH = NH_;
@@ -106,12 +110,16 @@ struct LaneTile {
   static constexpr int E = N >= L ? N / L : 1;            // after it
   static constexpr int kCopies = N >= L ? 1 : L / N;      // lanes that hold the same score
   static constexpr int HE = E < NH ? E : NH;              // different heads among a lane's scores
-  static constexpr int kScratch = TK * NH + NH;           // floats a warp
-  static constexpr int kVecs = sizeof(T) == 4 ? 2 : 1;    // 16-byte vectors of eight elements
+  // Floats a warp: each weight twice, as the operand of a multiplication of
+  // pairs, then a factor a head; in units of 16 bytes.
+  static constexpr int kScratch = 2 * TK * NH + (NH + 3) / 4 * 4;
+  static constexpr int kD = FULL ? 8 * L : 0;
+  static_assert(2 * TK * sizeof(T) >= NH * 4, "a warp's state fits into a stage");
 
   uint64_t q[NH][4], acc[NH][4];
   float m[HE], l[HE];
   int D, lane, l_id, group;
+  int key0, head0;  // of the first score that this lane holds after the exchange
   bool in0, in1;
 
   __host__ __device__ static int row_bytes(int D) { return D * (int)sizeof(T); }
@@ -120,29 +128,40 @@ struct LaneTile {
   __device__ __forceinline__ int elem(int i) const {  // element of slot i (0 .. 7) of this lane
     return sizeof(T) == 4 ? (i < 4 ? l_id * 4 + i : (l_id + L) * 4 + i - 4) : l_id * 8 + i;
   }
-  // First score (step * NH + head) that this lane holds after the exchange.
-  __device__ __forceinline__ int first_score() const { return N >= L ? l_id * E : l_id / kCopies; }
+  // Score e of this lane (step * NH + head counts them from n0): key and head.
+  __device__ __forceinline__ int key_of(int e) const { return key0 + e / NH * kKeysAtOnce; }
+  __device__ __forceinline__ int head_of(int e) const { return E < NH ? head0 + e : e % NH; }
 
-  __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t b, int h0, int nh) {
-    D = p.geom.head_dim;
-    lane = threadIdx.x % 32;
-    l_id = lane % L;
-    group = lane / L;
-    const int vecs = D * (int)sizeof(T) / 16;
-    in0 = l_id < vecs;
-    in1 = l_id + L < vecs;
+  template <class A>
+  __device__ __forceinline__ void load_q(const A* q0, int nh, float scale) {
 #pragma unroll
     for (int g = 0; g < NH; ++g) {
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = g < nh && elem(i) < D ? load_act(p.q, p.dt, b * p.q_stride + (int64_t)(h0 + g) * D + elem(i)) * p.scale : 0.f;
+      for (int i = 0; i < 8; ++i) x[i] = g < nh && elem(i) < D ? to_f(q0[g * D + elem(i)]) * scale : 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         q[g][i] = pack2(x[2 * i], x[2 * i + 1]);
         acc[g][i] = 0;
       }
     }
+  }
+
+  __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t b, int h0, int nh) {
+    D = FULL ? 8 * L : p.geom.head_dim;
+    lane = threadIdx.x % 32;
+    l_id = lane % L;
+    group = lane / L;
+    const int n0 = N >= L ? l_id * E : l_id / kCopies;
+    key0 = n0 / NH * kKeysAtOnce + group;
+    head0 = n0 % NH;
+    const int vecs = D * (int)sizeof(T) / 16;
+    in0 = FULL || l_id < vecs;
+    in1 = FULL || l_id + L < vecs;
+    const int64_t at = b * p.q_stride + (int64_t)h0 * D;
+    if (p.dt == DT_F32) load_q(static_cast<const float*>(p.q) + at, nh, p.scale);
+    else if (p.dt == DT_F16) load_q(static_cast<const __half*>(p.q) + at, nh, p.scale);
+    else load_q(static_cast<const __nv_bfloat16*>(p.q) + at, nh, p.scale);
 #pragma unroll
     for (int e = 0; e < HE; ++e) {
       m[e] = -INFINITY;
@@ -203,16 +222,18 @@ struct LaneTile {
         s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
       }
     }
-    const int n0 = first_score();
     float mx[HE];
 #pragma unroll
     for (int e = 0; e < HE; ++e) mx[e] = m[e];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int key = (n0 + e) / NH * kKeysAtOnce + group;
-      s[e] += add[key];
+      s[e] += add[key_of(e)];
       mx[e % HE] = fmaxf(mx[e % HE], s[e]);
-      if (scores && key < live && (n0 + e) % NH < nh) scores[key * group_size + (n0 + e) % NH] = s[e];
+    }
+    if (scores) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (key_of(e) < live && head_of(e) < nh) scores[key_of(e) * group_size + head_of(e)] = s[e];
     }
     // the maximum over the lanes that hold other keys of the same heads
 #pragma unroll
@@ -224,13 +245,13 @@ struct LaneTile {
 #pragma unroll
     for (int e = 0; e < HE; ++e) changed |= mx[e] != m[e];
     if (__any_sync(0xffffffffu, changed)) {
-      float* c = scratch + TK * NH;
+      float* c = scratch + 2 * TK * NH;
 #pragma unroll
       for (int e = 0; e < HE; ++e) {
         const float f = exp_from(m[e], mx[e]);
         l[e] *= f;
         m[e] = mx[e];
-        c[(n0 + e) % NH] = f;
+        c[head_of(e)] = f;
       }
       __syncwarp();
 #pragma unroll
@@ -240,31 +261,38 @@ struct LaneTile {
         for (int i = 0; i < 4; ++i) acc[g][i] = mul2(acc[g][i], f);
       }
     }
+    uint64_t* pairs = reinterpret_cast<uint64_t*>(scratch);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float x = exp_from(s[e], m[e % HE]);
       l[e % HE] += x;
-      scratch[((n0 + e) / NH * kKeysAtOnce + group) * NH + (n0 + e) % NH] = x;
+      pairs[key_of(e) * NH + head_of(e)] = pack2(x, x);
     }
     __syncwarp();
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
       const int key = st * kKeysAtOnce + group;
-      uint64_t x[4];
+      uint64_t x[4], f[NH];
       load_row(vs + key * rb, x);
+      if constexpr (NH == 1) {
+        f[0] = pairs[key];
+      } else {
 #pragma unroll
-      for (int g = 0; g < NH; ++g) {
-        const float f = scratch[key * NH + g];
-        const uint64_t ff = pack2(f, f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[g][i] = fma2(ff, x[i], acc[g][i]);
+        for (int g = 0; g < NH; g += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(pairs + key * NH + g);
+          f[g] = two.x;
+          f[g + 1] = two.y;
+        }
       }
+#pragma unroll
+      for (int g = 0; g < NH; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[g][i] = fma2(f[g], x[i], acc[g][i]);
     }
   }
 
   // The warp's state: ml[2 * head] the maximum, ml[2 * head + 1] the sum, o[head * D + d].
   __device__ __forceinline__ void dump(float* ml, float* o) {
-    const int n0 = first_score();
 #pragma unroll
     for (int off = 16; off; off >>= 1)
       if (off >= L || (off >= kCopies && off * E / kCopies >= NH))
@@ -272,8 +300,8 @@ struct LaneTile {
         for (int e = 0; e < HE; ++e) l[e] += __shfl_xor_sync(0xffffffffu, l[e], off);
 #pragma unroll
     for (int e = 0; e < HE; ++e) {
-      ml[2 * ((n0 + e) % NH)] = m[e];
-      ml[2 * ((n0 + e) % NH) + 1] = l[e];
+      ml[2 * head_of(e)] = m[e];
+      ml[2 * head_of(e) + 1] = l[e];
     }
 #pragma unroll
     for (int g = 0; g < NH; ++g) {
@@ -304,15 +332,18 @@ struct LaneTile {
 // fp16).  With up to eight heads hi takes rows 0-7 and lo rows 8-15 of the
 // same product.  D is padded to DT in shared memory; rows are swizzled by 16-byte
 // chunks so that ldmatrix reads eight rows without bank conflicts.
-template <class T_, int DT, int NH_>
+// With FULL, D is DT: no padding.
+template <class T_, int DT, int NH_, bool FULL>
 struct MmaTile {
   using T = T_;
   static constexpr int NH = NH_;
   static_assert(NH == 8 || NH == 16, "");
   static constexpr int TK = DT == 64 ? 32 : 16;
-  static constexpr int kStages = DT == 256 && NH == 16 ? 2 : 3;  // what shared memory holds beside the joint area
+  static constexpr int kStages = 3;
   static constexpr int kScratch = 0;
+  static constexpr int kD = FULL ? DT : 0;
   static constexpr int R = NH / 8;  // head rows of a thread
+  static_assert(2 * TK * DT * 2 >= NH * DT * 4, "a warp's state fits into a stage");
 
   uint32_t q[DT / 16][2 * R];
   float acc[DT / 8][4];
@@ -324,7 +355,7 @@ struct MmaTile {
   __device__ static __forceinline__ int chunk_at(int row, int chunk) { return chunk ^ (row & 7); }
 
   __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t b, int h0, int nh) {
-    D = p.geom.head_dim;
+    D = FULL ? DT : p.geom.head_dim;
     lane = threadIdx.x % 32;
     scale = p.scale;
     const T* base = static_cast<const T*>(p.q) + b * p.q_stride + (int64_t)h0 * D;
@@ -420,12 +451,16 @@ struct MmaTile {
         s[j][2 * r] = fmaf(s[j][2 * r], scale, a.x);
         s[j][2 * r + 1] = fmaf(s[j][2 * r + 1], scale, a.y);
         mx[r] = fmaxf(mx[r], fmaxf(s[j][2 * r], s[j][2 * r + 1]));
-        const int head = lane / 4 + 8 * r;
-        if (scores && head < nh) {
-          if (key < live) scores[key * group_size + head] = s[j][2 * r];
-          if (key + 1 < live) scores[(key + 1) * group_size + head] = s[j][2 * r + 1];
-        }
       }
+    }
+    if (scores) {
+#pragma unroll
+      for (int j = 0; j < TK / 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) {
+          const int key = j * 8 + lane % 4 * 2 + i % 2, head = lane / 4 + i / 2 * 8;
+          if (head < nh && key < live) scores[key * group_size + head] = s[j][i];
+        }
     }
     bool changed = false;
 #pragma unroll
@@ -520,14 +555,22 @@ __device__ __forceinline__ int tiles_of(int len) {  // an empty sequence takes o
   return len < 0 ? 0 : len == 0 ? 1 : (len + TILE - 1) / TILE;
 }
 
-// Shared memory in bytes: the warps' stages, their mask values, scratch and the states that are joined.
+// Shared memory in bytes: the warps' stages, their mask values and scratch.  At
+// the end of a segment a warp's state takes the place of the stage that it has just
+// used, which the next tile's load fills again: in all types NH * D floats fit
+// into the 2 * TK rows of a stage.
 template <class P>
 __host__ __device__ constexpr int attend_stage_bytes(int row_bytes) { return 2 * P::TK * row_bytes; }
 template <class P>
-inline int attend_smem(int row_bytes, int D) {
-  return kWarps * (P::kStages * (attend_stage_bytes<P>(row_bytes) + P::TK * 4) + P::kScratch * 4) +
-         kWarps * P::NH * (D + 2) * 4;
+inline int attend_smem(int row_bytes) {
+  return kWarps * (P::kStages * (attend_stage_bytes<P>(row_bytes) + P::TK * 4) + P::kScratch * 4);
 }
+
+// Parts of a segment that one block joins at a time: with more of them, groups
+// of neighbours are joined first, each by the last of its blocks, then the
+// groups (one block that reads 148 parts takes longer than the attention).
+constexpr int kMostParts = 32;
+static_assert(kMostParts * kMostParts >= kKvMaxBlocksPerSm * 256, "two levels cover the grid");
 
 template <class P>
 __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_constant__ KvAttendParams p) {
@@ -536,8 +579,10 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
   extern __shared__ __align__(128) char smem[];
   __shared__ long long s_warp[kWarps], s_base;
   __shared__ int s_b0, s_last;
+  __shared__ float s_ml[kWarps][NH][2];           // the warps' maxima and sums
+  __shared__ float s_part[kMostParts][NH], s_top[NH][2];  // a join: the parts' factors, the result's maximum and sum
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int D = p.geom.head_dim, kv = p.geom.kv_heads, group = p.heads / kv, chunks = (group + NH - 1) / NH;
+  const int D = P::kD ? P::kD : p.geom.head_dim, kv = p.geom.kv_heads, group = p.heads / kv, chunks = (group + NH - 1) / NH;
   const int per_tile = kv * chunks;  // segments of a sequence
 
   // The block's run of tiles: prefix sums of the sequences' tiles, each thread a slice of the batch.
@@ -615,13 +660,13 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
   char* ring = smem + warp * NS * stage_bytes;
   float* adds = reinterpret_cast<float*>(smem + kWarps * NS * stage_bytes) + warp * NS * TK;
   float* scratch = reinterpret_cast<float*>(smem + kWarps * NS * (stage_bytes + TK * 4)) + warp * P::kScratch;
-  float* joint = reinterpret_cast<float*>(smem + kWarps * (NS * (stage_bytes + TK * 4) + P::kScratch * 4));
-  if constexpr (P::kScratch == 0) {  // tensor cores read the padding of K up to DT: zeros, never written again
-    if (rb != D * (int)sizeof(T)) {
-      for (int i = lane; i < NS * stage_bytes / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
-      __syncwarp();
-    }
-  }
+  // Tensor cores read the padding of K rows up to DT, against zeros of q: it holds zeros, which no load overwrites.
+  const bool padded = !P::kD && rb != D * (int)sizeof(T);
+  auto clear = [&](char* at, int bytes) {
+    for (int i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  };
+  if (padded) clear(ring, NS * stage_bytes);
 
   // Fetching a tile: lane r holds the page and the mask value of the warp's row r.
   int f_page = -1;
@@ -631,7 +676,7 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
     f_page = -1;
     f_add = -INFINITY;
     if (lane < TK && i < c.len) {
-      const int col = i / p.geom.page_size;
+      const int col = p.page_shift >= 0 ? i >> p.page_shift : i / p.geom.page_size;
       f_page = col < p.table_cols ? p.table[c.b * p.table_stride + col] : -1;
       f_add = p.mask ? p.mask[c.b * p.mask_stride + i] : 0.f;
     }
@@ -651,7 +696,8 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
           set_status(p.status, ST_KV_PAGE);
           f_add = -INFINITY;
         } else {
-          off = row_offset(f_page, c.kvh, i % p.geom.page_size, p.geom) * (long long)sizeof(T);
+          const int slot = p.page_shift >= 0 ? i & ((1 << p.page_shift) - 1) : i % p.geom.page_size;
+          off = row_offset(f_page, c.kvh, slot, p.geom) * (long long)sizeof(T);
           fresh = p.k && i == c.len - 1;
         }
       }
@@ -662,6 +708,22 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
       // the new token's row is written below, unless the mask takes it out
       const int new_row = fresh_row ? __ffs(fresh_row) - 1 : 0;
       const bool put_new = fresh_row && __shfl_sync(0xffffffffu, f_add, new_row) != -INFINITY;
+      if (P::kD && __all_sync(0xffffffffu, off >= 0 || lane >= TK)) {
+        // whole rows of a known size: lane l takes vectors l, l + 32, ..
+        constexpr int V = P::kD ? P::kD * (int)sizeof(T) / 16 : 1;
+        const char* from = static_cast<const char*>(p.k_pages) + lane % V * 16;
+        const long long to_v = static_cast<const char*>(p.v_pages) - static_cast<const char*>(p.k_pages);
+        const uint32_t ka = smem_u32(ks), va = smem_u32(vs);
+#pragma unroll
+        for (int v = 0; v < TK * V; v += 32) {
+          const int row = V <= 32 ? v / V + lane / V : v / V, col = V <= 32 ? lane % V : v % V + lane;
+          const char* src = from + __shfl_sync(0xffffffffu, off, row) + (V <= 32 ? 0 : v % V * 16);
+          const int s = row * rb + P::chunk_at(row, col) * 16;
+          copy16(ka + s, src);
+          copy16(va + s, src + to_v);
+        }
+        return;
+      }
       int row = row_0, col = col_0;
       for (int v = 0; v < TK * vecs; v += 32) {
         const long long o = __shfl_sync(0xffffffffu, off, row & 31);
@@ -715,6 +777,7 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
   }
 
   P state;
+  int stage = 0, load_stage = NS - 1;  // of the tile in use, and of the next tile to load
   bool fresh_segment = true;
   long long seg_begin = t0 - use.tile;  // the segment's first tile
 #pragma unroll 1
@@ -725,16 +788,16 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
     copy_wait<NS - 2>();
     __syncwarp();
     if (issued < count) {
-      issue(load, issued % NS);
+      issue(load, load_stage);
       if (++issued < count) {
         advance(load);
         fetch(load);
       }
     }
     copy_commit();
+    load_stage = load_stage + 1 == NS ? 0 : load_stage + 1;
     const int first = use.tile * TILE + warp * TK;
     if (first < use.len) {
-      const int stage = j % NS;
       float* scores = p.weights_out
                           ? p.scores + (((long long)use.b * kv + use.kvh) * p.max_len + first) * group + use.chunk * NH
                           : nullptr;
@@ -744,78 +807,108 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
     const bool seg_end = use.tile + 1 == use.tiles;
     if (seg_end || j + 1 == count) {
       // join the warps
-      float* ml = joint;                   // [warp][NH][2]
-      float* o = joint + kWarps * NH * 2;  // [warp][NH][D]
-      state.dump(ml + warp * NH * 2, o + warp * NH * D);
+      const int stage_at = stage * stage_bytes;
+      state.dump(&s_ml[warp][0][0], reinterpret_cast<float*>(ring + stage_at));
       __syncthreads();
       const long long seg_last = seg_begin + use.tiles - 1;
       const bool whole = seg_begin >= t0 && seg_end;
-      const int slot = seg_begin <= t0 ? 0 : 1;
-      float* part = p.parts + (2ll * blockIdx.x + slot) * NH * (D + 2);
-      for (int x = tid; x < nh * D; x += kThreads) {
+      auto part_at = [&](long long slot) { return p.parts + slot * NH * (D + 2); };  // [NH][2], then [nh][D]
+      auto finish = [&](int x, float mt, float lt, float ot) {
         const int h = x / D, d = x % D;
+        store_act(p.out, p.dt, use.b * p.out_stride + (int64_t)h0 * D + x, lt != 0.f ? ot / lt : 0.f);
+        if (p.weights_out && d == 0) {
+          p.stats[((int64_t)use.b * p.heads + h0 + h) * 2] = mt;
+          p.stats[((int64_t)use.b * p.heads + h0 + h) * 2 + 1] = lt;
+        }
+      };
+      long long slot = 2ll * blockIdx.x + (seg_begin <= t0 ? 0 : 1);
+      for (int x = tid; x < nh * D; x += kThreads) {
+        const int h = x / D;
         float mt = -INFINITY, lt = 0.f, ot = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, ml[(w * NH + h) * 2]);
+        for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, s_ml[w][h][0]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float c = exp_from(ml[(w * NH + h) * 2], mt);
-          lt += ml[(w * NH + h) * 2 + 1] * c;
-          ot += o[(w * NH + h) * D + d] * c;
+          const float c = exp_from(s_ml[w][h][0], mt);
+          lt += s_ml[w][h][1] * c;
+          ot += reinterpret_cast<const float*>(smem + w * NS * stage_bytes + stage_at)[x] * c;
         }
         if (whole) {
-          store_act(p.out, p.dt, use.b * p.out_stride + (int64_t)(h0 + h) * D + d, lt != 0.f ? ot / lt : 0.f);
-          if (p.weights_out && d == 0) {
-            p.stats[((int64_t)use.b * p.heads + h0 + h) * 2] = mt;
-            p.stats[((int64_t)use.b * p.heads + h0 + h) * 2 + 1] = lt;
-          }
+          finish(x, mt, lt, ot);
         } else {
-          part[2 * NH + x] = ot;
-          if (d == 0) {
-            part[2 * h] = mt;
-            part[2 * h + 1] = lt;
+          part_at(slot)[2 * NH + x] = ot;
+          if (x % D == 0) {
+            part_at(slot)[2 * h] = mt;
+            part_at(slot)[2 * h + 1] = lt;
           }
         }
       }
       if (!whole) {
-        // block that holds tile t: the largest i with floor(total * i / blocks) <= t
+        // The segment's blocks are c0 .. c1; the one that holds tile t is the
+        // largest i with floor(total * i / blocks) <= t.  Block c left its part in its slot 0, or
+        // c0, where an earlier segment took that, in slot 1.
         const int c0 = (int)(((seg_begin + 1) * blocks - 1) / total);
-        const int c1 = (int)(((seg_last + 1) * blocks - 1) / total);
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          // wraps to 0 with the last arrival: ready for the next call
-          const unsigned old = atomicInc(p.arrived + ((int64_t)use.b * kv + use.kvh) * chunks + use.chunk, c1 - c0);
-          s_last = old == (unsigned)(c1 - c0);
-        }
-        __syncthreads();
-        if (s_last) {
+        const int n = (int)(((seg_last + 1) * blocks - 1) / total) - c0 + 1;
+        const long long base = 2ll * c0, first_slot = base + (total * c0 / blocks >= seg_begin ? 0 : 1);
+        int fan = 8;  // parts of a group
+        while (fan * fan < n) fan *= 2;
+        const int me = blockIdx.x - c0;
+        for (int level = 0, step = 1; level < 2; ++level, step = fan) {
+          // this block's group: parts lo, lo + step, .. below hi; it is complete with its last arrival
+          const int lo = level == 0 ? me / fan * fan : 0, hi = level == 0 ? min(lo + fan, n) : n;
+          const int k = (hi - lo + step - 1) / step;
+          if (level == 1 && n <= fan) break;
+          auto slot_of = [&](int i) { return i == 0 ? first_slot : base + 2ll * i; };
           __threadfence();
-          const bool c0_first = total * c0 / blocks >= seg_begin;  // the segment is the first of block c0's run
-          auto part_of = [&](int c) { return p.parts + (2ll * c + (c == c0 && !c0_first ? 1 : 0)) * NH * (D + 2); };
-          for (int x = tid; x < nh * D; x += kThreads) {
-            const int h = x / D, d = x % D;
-            float mt = -INFINITY, lt = 0.f, ot = 0.f;
-            for (int c = c0; c <= c1; ++c) mt = fmaxf(mt, __ldcg(part_of(c) + 2 * h));
-            for (int c = c0; c <= c1; ++c) {
-              const float* q = part_of(c);
-              const float f = exp_from(__ldcg(q + 2 * h), mt);
-              lt += __ldcg(q + 2 * h + 1) * f;
-              ot += __ldcg(q + 2 * NH + x) * f;
+          __syncthreads();
+          if (tid == 0)  // the counter wraps to 0 with the last arrival: ready for the next call
+            s_last = k == 1 || atomicInc(p.arrived + 2 * slot_of(lo) + level, k - 1) == (unsigned)(k - 1);
+          __syncthreads();
+          if (!s_last) break;
+          __threadfence();
+          if (k == 1) continue;
+          for (int h = warp; h < nh; h += kWarps) {
+            const float* q = part_at(slot_of(lo + min(lane, k - 1) * step));
+            const float m = lane < k ? __ldcg(q + 2 * h) : -INFINITY, l = lane < k ? __ldcg(q + 2 * h + 1) : 0.f;
+            float mt = m;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+            const float f = exp_from(m, mt);
+            float lt = l * f;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+            s_part[lane][h] = f;
+            if (lane == 0) {
+              s_top[h][0] = mt;
+              s_top[h][1] = lt;
             }
-            store_act(p.out, p.dt, use.b * p.out_stride + (int64_t)(h0 + h) * D + d, lt != 0.f ? ot / lt : 0.f);
-            if (p.weights_out && d == 0) {
-              p.stats[((int64_t)use.b * p.heads + h0 + h) * 2] = mt;
-              p.stats[((int64_t)use.b * p.heads + h0 + h) * 2 + 1] = lt;
+          }
+          __syncthreads();
+          const bool done = level == 1 || n <= fan;
+          for (int x = tid; x < nh * D; x += kThreads) {
+            const int h = x / D;
+            float ot = 0.f;
+#pragma unroll 8
+            for (int i = 0; i < k; ++i) ot += __ldcg(part_at(slot_of(lo + i * step)) + 2 * NH + x) * s_part[i][h];
+            if (done) {
+              finish(x, s_top[h][0], s_top[h][1], ot);
+            } else {  // in place of the group's first part, which no other block reads any more
+              part_at(slot_of(lo))[2 * NH + x] = ot;
+              if (x % D == 0) {
+                part_at(slot_of(lo))[2 * h] = s_top[h][0];
+                part_at(slot_of(lo))[2 * h + 1] = s_top[h][1];
+              }
             }
           }
         }
       }
-      __syncthreads();  // the joint area is free again
+      __syncthreads();  // the stages are free again
+      if (padded) clear(ring + stage_at, stage_bytes);
       if (j + 1 < count) seg_begin = seg_last + 1;
       fresh_segment = true;
     }
     if (j + 1 < count) advance(use);
+    stage = stage + 1 == NS ? 0 : stage + 1;
   }
   copy_wait<0>();
   if (blockIdx.x == 0)  // lengths that length_of took as 0
@@ -847,42 +940,47 @@ cudaError_t blocks_per_sm(int device, int smem, int* out) {
 
 template <class P>
 cudaError_t attend_launch(const KvAttendParams& p, cudaStream_t s) {
-  const int D = p.geom.head_dim, smem = attend_smem<P>(P::row_bytes(D), D);
+  const int D = p.geom.head_dim, smem = attend_smem<P>(P::row_bytes(D));
   int per_sm = 0;
   if (cudaError_t e = blocks_per_sm<P>(p.device, smem, &per_sm)) return e;
   kv_attend_kernel<P><<<p.sms * per_sm, kThreads, smem, s>>>(p);
   return cudaGetLastError();
 }
 
-// The lanes' kernel for this head dim and group.
-template <class T, int L>
-cudaError_t attend_lanes_l(const KvAttendParams& p, cudaStream_t s) {
+// The kernel for these types, head dim and group.
+template <class T, int L, bool FULL>
+cudaError_t attend_lanes_group(const KvAttendParams& p, cudaStream_t s) {
   const int group = p.heads / p.geom.kv_heads;
-  if (group <= 1) return attend_launch<LaneTile<T, L, 1>>(p, s);
-  if (group <= 2) return attend_launch<LaneTile<T, L, 2>>(p, s);
-  if (group <= 4) return attend_launch<LaneTile<T, L, 4>>(p, s);
-  return attend_launch<LaneTile<T, L, 8>>(p, s);
+  if (group <= 1) return attend_launch<LaneTile<T, L, 1, FULL>>(p, s);
+  if (group <= 2) return attend_launch<LaneTile<T, L, 2, FULL>>(p, s);
+  // a stage of four 16-bit rows has no room for the states of eight heads
+  constexpr int kMost = L == 32 && sizeof(T) == 2 ? 4 : 8;
+  if (group <= 4) return attend_launch<LaneTile<T, L, 4, FULL>>(p, s);
+  return attend_launch<LaneTile<T, L, kMost, FULL>>(p, s);
 }
 template <class T>
 cudaError_t attend_lanes(const KvAttendParams& p, cudaStream_t s) {
   const int D = p.geom.head_dim;
-  if (D <= 32) return attend_lanes_l<T, 4>(p, s);
-  if (D <= 64) return attend_lanes_l<T, 8>(p, s);
-  if (D <= 128) return attend_lanes_l<T, 16>(p, s);
-  return attend_lanes_l<T, 32>(p, s);
+  if (D <= 32) return attend_lanes_group<T, 4, false>(p, s);
+  if (D < 64) return attend_lanes_group<T, 8, false>(p, s);
+  if (D == 64) return attend_lanes_group<T, 8, true>(p, s);
+  if (D < 128) return attend_lanes_group<T, 16, false>(p, s);
+  if (D == 128) return attend_lanes_group<T, 16, true>(p, s);
+  return attend_lanes_group<T, 32, false>(p, s);
 }
 template <class T, int NH>
 cudaError_t attend_mma(const KvAttendParams& p, cudaStream_t s) {
   const int D = p.geom.head_dim;
-  if (D <= 64) return attend_launch<MmaTile<T, 64, NH>>(p, s);
-  if (D <= 128) return attend_launch<MmaTile<T, 128, NH>>(p, s);
-  return attend_launch<MmaTile<T, 256, NH>>(p, s);
+  if (D < 64) return attend_launch<MmaTile<T, 64, NH, false>>(p, s);
+  if (D == 64) return attend_launch<MmaTile<T, 64, NH, true>>(p, s);
+  if (D < 128) return attend_launch<MmaTile<T, 128, NH, false>>(p, s);
+  if (D == 128) return attend_launch<MmaTile<T, 128, NH, true>>(p, s);
+  return attend_launch<MmaTile<T, 256, NH, false>>(p, s);
 }
 template <class T>
 cudaError_t attend_16bit(const KvAttendParams& p, cudaStream_t s) {
   const int group = p.heads / p.geom.kv_heads;
-  if (p.dt == TypeCode<T>::value && group > 1)
-    return group <= 8 ? attend_mma<T, 8>(p, s) : attend_mma<T, 16>(p, s);
+  if (p.dt == TypeCode<T>::value && group > 1) return group <= 8 ? attend_mma<T, 8>(p, s) : attend_mma<T, 16>(p, s);
   return attend_lanes<T>(p, s);
 }
 

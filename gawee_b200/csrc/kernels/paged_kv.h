@@ -10,10 +10,10 @@
 namespace gawee {
 namespace kern {
 
-// Attention: query heads of a key/value head that a block computes together at
-// most (a larger group takes several runs over the same keys) and at least, and
-// the blocks that an SM holds at most.  They size the workspace.
-constexpr int kKvHeadsMost = 16, kKvHeadsLeast = 8, kKvMaxBlocksPerSm = 4;
+// Attention: the query heads of a key/value head that a block computes together
+// at most (a larger group takes several runs over the same keys) and the blocks
+// that an SM holds at most.  They size the workspace.
+constexpr int kKvHeadsMost = 16, kKvMaxBlocksPerSm = 4;
 
 // Rows of new tokens into the pages: token t's key k[t * k_stride + h * D ..]
 // goes to row positions[t] of sequence sequences[t] (nullptr: sequence t).  A
@@ -59,8 +59,9 @@ struct KvAttendParams {
   float* scores;         // [batch][kv_heads][max_len][heads / kv_heads], with weights_out
   float* stats;          // [batch][heads][2]: maximum and sum, with weights_out
   float* parts;          // states of parts of segments: two a block, heads of a block * (D + 2) each
-  unsigned* arrived;     // [batch][kv_heads][chunks of heads] parts that are there; 0 between calls
+  unsigned* arrived;     // two counters of arrivals a part; 0 between calls
   int device, sms;
+  int page_shift;        // log2 of the page size, -1 where it is no power of two
   int* status;
 };
 cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s);
