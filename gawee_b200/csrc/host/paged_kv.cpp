@@ -19,7 +19,7 @@ struct gawee_kv {
   gawee::kern::PageGeom geom{};
   int device = -1;
   int* status = nullptr;       // first error a kernel reported (kern::Status)
-  int32_t* new_len = nullptr;  // [max_batch]
+  int32_t* plan = nullptr;     // [max_batch][2]: evict's lengths before and after
   float* stats = nullptr;      // [max_batch][heads][2], with desc.weights
   float* scores = nullptr;     // [max_batch][heads][max_pages * page_size], with desc.weights
   float* parts = nullptr;      // attend's partial states
@@ -27,7 +27,7 @@ struct gawee_kv {
   int sms = 0;
   ~gawee_kv() {
     cudaFree(status);
-    cudaFree(new_len);
+    cudaFree(plan);
     cudaFree(stats);
     cudaFree(scores);
     cudaFree(parts);
@@ -164,7 +164,7 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     e = scope.err;
     const size_t rows = (size_t)d.max_batch * d.heads;
     if (e == cudaSuccess) e = cudaMalloc((void**)&kv->status, sizeof(int));
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->new_len, sizeof(int32_t) * d.max_batch);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->plan, sizeof(int32_t) * 2 * d.max_batch);
     if (e == cudaSuccess && d.weights) e = cudaMalloc((void**)&kv->stats, sizeof(float) * 2 * rows);
     if (e == cudaSuccess && d.weights)
       e = cudaMalloc((void**)&kv->scores, sizeof(float) * rows * d.max_pages * d.page_size);
@@ -375,7 +375,8 @@ gawee_status gawee_kv_evict(gawee_kv* kv, const gawee_kv_evict_args* a, void* st
     p.budget = a->budget;
     p.recent = a->recent;
     p.kept = a->kept;
-    p.new_len = kv->new_len;
+    p.plan = kv->plan;
+    p.sms = kv->sms;
     p.status = kv->status;
     return run_on(kv, kName, [&] { return launch_kv_evict(p, static_cast<cudaStream_t>(stream)); });
   });

@@ -105,7 +105,7 @@ struct LaneTile {
   static constexpr int TK = kSteps * kKeysAtOnce;  // keys of a warp's tile
   // A stage holds K and V rows of at most TK * 8 L elements: 8 KB in fp32, 4 KB
   // in 16 bits.  Two blocks of four warps on an SM then have about 128 KB on the way.
-  static constexpr int kStages = sizeof(T) == 4 ? 3 : 6;
+  static constexpr int kStages = (NH <= 4 ? 2 : 3) * (sizeof(T) == 4 ? 1 : 2);
   static constexpr int N = kSteps * NH;                   // scores of a lane before the exchange
   static constexpr int E = N >= L ? N / L : 1;            // after it
   static constexpr int kCopies = N >= L ? 1 : L / N;      // lanes that hold the same score
@@ -708,19 +708,38 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
       // the new token's row is written below, unless the mask takes it out
       const int new_row = fresh_row ? __ffs(fresh_row) - 1 : 0;
       const bool put_new = fresh_row && __shfl_sync(0xffffffffu, f_add, new_row) != -INFINITY;
-      if (P::kD && __all_sync(0xffffffffu, off >= 0 || lane >= TK)) {
-        // whole rows of a known size: lane l takes vectors l, l + 32, ..
-        constexpr int V = P::kD ? P::kD * (int)sizeof(T) / 16 : 1;
-        const char* from = static_cast<const char*>(p.k_pages) + lane % V * 16;
-        const long long to_v = static_cast<const char*>(p.v_pages) - static_cast<const char*>(p.k_pages);
+      if (__all_sync(0xffffffffu, off >= 0 || lane >= TK)) {  // whole rows: lane l takes vectors l, l + 32, ..
+        const char* from = static_cast<const char*>(p.k_pages);
+        const long long to_v = static_cast<const char*>(p.v_pages) - from;
         const uint32_t ka = smem_u32(ks), va = smem_u32(vs);
+        if constexpr (P::kD != 0) {
+          constexpr int V = P::kD * (int)sizeof(T) / 16;
+          from += lane % V * 16;
 #pragma unroll
-        for (int v = 0; v < TK * V; v += 32) {
-          const int row = V <= 32 ? v / V + lane / V : v / V, col = V <= 32 ? lane % V : v % V + lane;
-          const char* src = from + __shfl_sync(0xffffffffu, off, row) + (V <= 32 ? 0 : v % V * 16);
-          const int s = row * rb + P::chunk_at(row, col) * 16;
-          copy16(ka + s, src);
-          copy16(va + s, src + to_v);
+          for (int v = 0; v < TK * V; v += 32) {
+            const int row = V <= 32 ? v / V + lane / V : v / V, col = V <= 32 ? lane % V : v % V + lane;
+            const char* src = from + __shfl_sync(0xffffffffu, off, row) + (V <= 32 ? 0 : v % V * 16);
+            const int s = row * rb + P::chunk_at(row, col) * 16;
+            copy16(ka + s, src);
+            copy16(va + s, src + to_v);
+          }
+        } else {
+          int row = row_0, col = col_0;
+#pragma unroll 4
+          for (int v = 0; v < TK * vecs; v += 32) {
+            const char* src = from + __shfl_sync(0xffffffffu, off, row & 31) + col * 16;
+            const int s = row * rb + P::chunk_at(row, col) * 16;
+            if (row < TK) {
+              copy16(ka + s, src);
+              copy16(va + s, src + to_v);
+            }
+            row += row_step;
+            col += col_step;
+            if (col >= vecs) {
+              col -= vecs;
+              ++row;
+            }
+          }
         }
         return;
       }

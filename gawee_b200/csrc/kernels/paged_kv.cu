@@ -1,6 +1,8 @@
 // Kernels of the paged key/value cache: append, the weights' pass of
 // attend (the attention itself is in paged_attend.cuh) and eviction by
 // accumulated attention weight.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cstdint>
 
@@ -14,51 +16,107 @@ using namespace paged;
 namespace {
 
 // --- append -------------------------------------------------------------------
-// One thread per element of a token's row over the heads.
-template <class T>
-__global__ void kv_append_kernel(KvAppendParams p) {
-  const int row = p.geom.kv_heads * p.geom.head_dim;
-  for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    const int64_t seq = p.sequences ? (int64_t)p.sequences[t] : t;
-    const int64_t pos = p.positions[t];
-    if (seq < 0 || pos < 0) continue;
-    const int64_t page = seq < p.batch ? page_of(p.table + seq * p.table_stride, p.table_cols, pos, p.geom) : -1;
-    if (page < 0) {
-      if (threadIdx.x == 0) set_status(p.status, seq < p.batch ? ST_KV_PAGE : ST_KV_SEQUENCE);
-      continue;
+// A thread takes 16-byte vectors of a token's row over the heads, of K and of V.
+// The bound is HBM bandwidth; the chain position -> page -> row is short, and
+// many tokens are on the way at once.
+constexpr int kAppendThreads = 256;
+
+// `n` consecutive values as fp32; 16-byte loads where the caller knows the alignment.
+template <class A, int N, bool ALIGNED>
+__device__ __forceinline__ void load_n(const A* p, float (&x)[N]) {
+  if constexpr (ALIGNED) {
+    constexpr int kPer = 16 / sizeof(A), kV = N >= kPer ? N / kPer : 1;
+    if constexpr (N >= kPer) {
+#pragma unroll
+      for (int v = 0; v < kV; ++v) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p + v * kPer);
+        const A* e = reinterpret_cast<const A*>(&a);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[v * kPer + i] = to_f(e[i]);
+      }
+    } else {  // four 16-bit values: 8 bytes
+      const uint2 a = *reinterpret_cast<const uint2*>(p);
+      const A* e = reinterpret_cast<const A*>(&a);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = to_f(e[i]);
     }
-    const int slot = (int)(pos % p.geom.page_size);
-    for (int i = threadIdx.x; i < row; i += blockDim.x) {
-      const int h = i / p.geom.head_dim, d = i % p.geom.head_dim;
-      const int64_t o = row_offset(page, h, slot, p.geom) + d;
-      static_cast<T*>(p.k_pages)[o] = from_f<T>(load_act(p.k, p.dt, t * p.k_stride + i));
-      static_cast<T*>(p.v_pages)[o] = from_f<T>(load_act(p.v, p.dt, t * p.v_stride + i));
-    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_f(p[i]);
   }
 }
 
+template <class T, class A, bool ALIGNED>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendParams p, int lanes) {
+  constexpr int kPer = 16 / sizeof(T);
+  const int64_t t = (int64_t)blockIdx.x * (kAppendThreads / lanes) + threadIdx.x / lanes;
+  if (t >= p.tokens) return;
+  const int64_t seq = p.sequences ? (int64_t)p.sequences[t] : t;
+  const int64_t pos = p.positions[t];
+  if (seq < 0 || pos < 0) return;
+  const int lane = threadIdx.x % lanes, head_vecs = p.geom.head_dim / kPer, vecs = p.geom.kv_heads * head_vecs;
+  const int64_t page = seq < p.batch ? page_of(p.table + seq * p.table_stride, p.table_cols, pos, p.geom) : -1;
+  if (page < 0) {
+    if (lane == 0) set_status(p.status, seq < p.batch ? ST_KV_PAGE : ST_KV_SEQUENCE);
+    return;
+  }
+  const int slot = (int)(pos % p.geom.page_size);
+  const A *k = static_cast<const A*>(p.k) + t * p.k_stride, *v = static_cast<const A*>(p.v) + t * p.v_stride;
+  for (int i = lane; i < vecs; i += lanes) {
+    const int64_t o = row_offset(page, i / head_vecs, slot, p.geom) + i % head_vecs * kPer;
+    float x[kPer], y[kPer];
+    load_n<A, kPer, ALIGNED>(k + i * kPer, x);
+    load_n<A, kPer, ALIGNED>(v + i * kPer, y);
+    uint4 a, b;
+    T *ka = reinterpret_cast<T*>(&a), *va = reinterpret_cast<T*>(&b);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      ka[e] = from_f<T>(x[e]);
+      va[e] = from_f<T>(y[e]);
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.k_pages) + o) = a;
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.v_pages) + o) = b;
+  }
+}
+
+// --- the weights of attend ------------------------------------------------------
 // weights_out = weights + the attention weights of this step, summed over the
-// query heads of the key/value head in their order.
-__global__ void kv_weights_kernel(KvAttendParams p) {
+// query heads of the key/value head in their order.  Bound by the scores and
+// accumulators it reads and writes, which the attention left in L2.
+constexpr int kWeightThreads = 256;
+
+__global__ void __launch_bounds__(kWeightThreads) kv_weights_kernel(KvAttendParams p) {
+  extern __shared__ float2 s_head[];  // maximum and 1 / sum of each query head of the group
   const int kvh = blockIdx.x % p.geom.kv_heads, b = blockIdx.x / p.geom.kv_heads;
   const int group = p.heads / p.geom.kv_heads;
   const int64_t len = p.lengths[b];
-  if (len > p.max_len) return;
+  if (len > p.max_len || (int64_t)blockIdx.y * kWeightThreads >= len) return;
   const float* stats = p.stats + ((int64_t)b * p.heads + kvh * group) * 2;
-  for (int64_t i = (int64_t)blockIdx.y * blockDim.x + threadIdx.x; i < len; i += (int64_t)gridDim.y * blockDim.x) {
+  for (int g = threadIdx.x; g < group; g += kWeightThreads) s_head[g] = make_float2(stats[2 * g], 1.f / stats[2 * g + 1]);
+  __syncthreads();
+  for (int64_t i = (int64_t)blockIdx.y * kWeightThreads + threadIdx.x; i < len; i += (int64_t)gridDim.y * kWeightThreads) {
     const float* s = p.scores + ((int64_t)blockIdx.x * p.max_len + i) * group;
+    const float before = p.weights ? p.weights[b * p.w_batch + kvh * p.w_stride + i] : 0.f;
     float w = 0.f;
     for (int g = 0; g < group; ++g) {
-      const float m = stats[2 * g], l = stats[2 * g + 1];
-      w += s[g] == -INFINITY ? 0.f : exp2f((s[g] - m) * kLog2e) / l;
+      const float2 h = s_head[g];
+      w += s[g] == -INFINITY ? 0.f : exp2f((s[g] - h.x) * kLog2e) * h.y;
     }
-    const float before = p.weights ? p.weights[b * p.w_batch + kvh * p.w_stride + i] : 0.f;
     p.weights_out[b * p.wo_batch + kvh * p.wo_stride + i] = before + w;
   }
 }
 
 // --- evict ---------------------------------------------------------------------
+//
+// Selection: a cluster of blocks per (sequence, key/value head), each a
+// contiguous range of the positions.  The smallest weight that stays is found
+// by radix selection over the bits of weight_key, 11 + 11 + 10 of them, with
+// the blocks' histograms summed through distributed shared memory; equal
+// weights stay from the lowest position on, so a kept row's new place is
+//   (kept for certain before it) + min(equal before it, equal ones that stay).
+// The weights are read five times, the first time from HBM, and the bound is the latency of the passes.
 constexpr int kSelectThreads = 1024;
+constexpr int kBins = 2048;
 
 // Weights in ascending order of their values as unsigned integers; both zeros
 // are equal and NaN is below every number.
@@ -68,133 +126,234 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Inclusive sums over the block of two flags; every thread calls it.
-__device__ __forceinline__ int2 block_scan(int a, int b, int2* warp_sums, int2& total) {
+// Sums of x over the block's threads before this one, and over all; every thread calls it.
+__device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  int packed = a | (b << 16);
+  int scan = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, packed, o);
-    if (lane >= o) packed += up;
+    const int up = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += up;
   }
+  __syncthreads();  // the last call's sums have been read
+  if (lane == 31) warp_sums[warp] = scan;
   __syncthreads();
-  if (lane == 31) warp_sums[warp] = make_int2(packed & 0xffff, packed >> 16);
-  __syncthreads();
-  int2 before = make_int2(0, 0);
-  total = make_int2(0, 0);
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    if (w == warp) before = total;
-    total.x += warp_sums[w].x;
-    total.y += warp_sums[w].y;
+  const int mine = warp_sums[lane];  // as many warps as lanes
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += up;
   }
-  return make_int2(before.x + (packed & 0xffff), before.y + (packed >> 16));
+  total = __shfl_sync(0xffffffffu, upto, 31);
+  const int before = __shfl_sync(0xffffffffu, upto - mine, warp);
+  return before + scan - x;
 }
+static_assert(kSelectThreads == 32 * 32, "block_scan takes one warp's lanes for the warps");
 
-// One block per (sequence, key/value head): the smallest weight that stays, by
-// radix selection over the bits of weight_key, then the kept positions in
-// order, with their weights moved to the front.
 __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams p) {
-  __shared__ int hist[256];
-  __shared__ int2 warp_sums[kSelectThreads / 32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
-  const int kvh = blockIdx.x % p.geom.kv_heads, b = blockIdx.x / p.geom.kv_heads;
-  int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
-  int64_t len = p.lengths[b];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  __shared__ int hist[2][kBins];
+  __shared__ int warp_sums[32];
+  __shared__ int s_bin, s_need, s_sure, s_equal;
+  const int pair = blockIdx.x / blocks;
+  const int kvh = pair % p.geom.kv_heads, b = pair / p.geom.kv_heads;
+  const int tid = threadIdx.x;
+  int32_t* kept = p.kept + (int64_t)pair * p.budget;
+  int len = p.lengths[b];
   if (len > p.max_len) {
-    if (threadIdx.x == 0) set_status(p.status, ST_KV_LENGTH);
+    if (tid == 0) set_status(p.status, ST_KV_LENGTH);
     len = -1;
   }
-  const bool first = kvh == 0 && threadIdx.x == 0;
-  if (first) p.new_len[b] = len > p.budget ? p.budget : p.lengths[b];
-  const float* w = p.weights + b * p.w_batch + kvh * p.w_stride;
-  float* wo = p.weights_out + b * p.wo_batch + kvh * p.wo_stride;
-  if (len <= p.budget) {
-    for (int j = threadIdx.x; j < p.budget; j += kSelectThreads) kept[j] = j < len ? j : -1;
-    for (int j = threadIdx.x; j < len; j += kSelectThreads) wo[j] = w[j];
+  if (kvh == 0 && rank == 0 && tid == 0) {
+    p.plan[2 * b] = len;
+    p.plan[2 * b + 1] = len > p.budget ? p.budget : p.lengths[b];
+  }
+  if (len <= p.budget) {  // the whole cluster
+    for (int j = rank * kSelectThreads + tid; j < p.budget; j += blocks * kSelectThreads) kept[j] = j < len ? j : -1;
     return;
   }
-  const int cand = (int)len - p.recent;
+  const float* w = p.weights + b * p.w_batch + kvh * p.w_stride;
+  const int cand = len - p.recent;  // positions below it are chosen by weight
+  const int range = (len + blocks - 1) / blocks, begin = min(rank * range, len), end = min(begin + range, len);
+  const int old_end = min(end, cand);
   uint32_t prefix = 0;
   int need = p.budget - p.recent;  // still to choose among the keys with this prefix
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kSelectThreads) hist[i] = 0;
+  const bool choose = need > 0;
+  for (int pass = 0; pass < 3 && choose; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    const uint32_t above = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
+    int* mine = hist[pass & 1];
+    for (int i = tid; i < kBins; i += kSelectThreads) mine[i] = 0;
     __syncthreads();
-    const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int i = threadIdx.x; i < cand; i += kSelectThreads) {
-      const uint32_t k = weight_key(w[i]);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+    for (int base = begin; base < old_end; base += kSelectThreads) {
+      const int i = base + tid;
+      const uint32_t k = i < old_end ? weight_key(w[i]) : 0u;
+      const bool in = i < old_end && (k & above) == prefix;
+      const int bin = in ? (int)((k >> shift) & ((1u << bits) - 1)) : -1;
+      int same;
+      __match_all_sync(0xffffffffu, bin, &same);
+      if (same) {  // many equal weights: one addition for the warp
+        if (bin >= 0 && tid % 32 == 0) atomicAdd(&mine[bin], 32);
+      } else if (bin >= 0) {
+        atomicAdd(&mine[bin], 1);
+      }
+    }
+    cluster.sync();
+    // this thread's two bins, from the highest down
+    const int hi = kBins - 1 - 2 * tid, lo = hi - 1;
+    int h1 = 0, h0 = 0;
+    for (int r = 0; r < blocks; ++r) {
+      const int* theirs = cluster.map_shared_rank(mine, r);
+      h1 += theirs[hi];
+      h0 += theirs[lo];
+    }
+    int total;
+    const int before = block_scan(h1 + h0, warp_sums, total);
+    if (before < need && before + h1 >= need) {
+      s_bin = hi;
+      s_need = need - before;
+    } else if (before + h1 < need && before + h1 + h0 >= need) {
+      s_bin = lo;
+      s_need = need - before - h1;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      int bin = 255, n = need;
-      while (hist[bin] < n) n -= hist[bin--];
-      s_prefix = prefix | ((uint32_t)bin << shift);
-      s_need = n;
-    }
-    __syncthreads();
-    prefix = s_prefix;
+    prefix |= (uint32_t)s_bin << shift;
     need = s_need;
+    // a block clears this histogram again only two passes on, behind the next cluster.sync
   }
-  // keys above `prefix` stay, and the first `need` of those equal to it
-  const bool none = p.budget == p.recent;
-  int out = 0, equal = 0;
-  for (int base = 0; base < len; base += kSelectThreads) {
-    const int i = base + threadIdx.x;
-    const float x = i < len ? w[i] : 0.f;
-    const uint32_t k = weight_key(x);
-    const bool old = i < cand && !none;
-    const bool eq = old && k == prefix;
-    int2 total;
-    const int2 e = block_scan(eq, 0, warp_sums, total);
-    const bool keep = i < len && (i >= cand || (old && (k > prefix || (eq && equal + e.x <= need))));
-    equal += total.x;
-    const int2 r = block_scan(keep, 0, warp_sums, total);
-    if (keep) {
-      kept[out + r.x - 1] = i;
-      wo[out + r.x - 1] = x;
+  // keys above `prefix` and the recent rows stay for certain, and the first `need` of those equal to it
+  auto classify = [&](int i, int& sure, int& equal) {
+    sure = i < end && i >= cand;
+    equal = 0;
+    if (choose && i < old_end) {
+      const uint32_t k = weight_key(w[i]);
+      sure = k > prefix;
+      equal = k == prefix;
     }
-    out += total.x;
+  };
+  int sure = 0, equal = 0;
+  for (int i = begin + tid; i < end; i += kSelectThreads) {
+    int a, e;
+    classify(i, a, e);
+    sure += a;
+    equal += e;
   }
-  for (int i = p.budget + threadIdx.x; i < len; i += kSelectThreads) wo[i] = 0.f;
+  int all_sure, all_equal;
+  block_scan(sure, warp_sums, all_sure);
+  block_scan(equal, warp_sums, all_equal);
+  if (tid == 0) {
+    s_sure = all_sure;
+    s_equal = all_equal;
+  }
+  cluster.sync();
+  int sure_before = 0, equal_before = 0;
+  for (int r = 0; r < rank; ++r) {
+    sure_before += *cluster.map_shared_rank(&s_sure, r);
+    equal_before += *cluster.map_shared_rank(&s_equal, r);
+  }
+  cluster.sync();  // no block leaves while its shared memory is read
+  constexpr int kEach = 4;  // consecutive positions of a thread
+  for (int base = begin; base < end; base += kSelectThreads * kEach) {
+    int a[kEach], e[kEach], packed = 0;
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+      classify(base + tid * kEach + x, a[x], e[x]);
+      packed += a[x] | e[x] << 16;
+    }
+    int total;
+    const int before = block_scan(packed, warp_sums, total);
+    int s = sure_before + (before & 0xffff), q = equal_before + (before >> 16);
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+      if (a[x] || (e[x] && q < need)) kept[s + min(q, need)] = base + tid * kEach + x;
+      s += a[x];
+      q += e[x];
+    }
+    sure_before += total & 0xffff;
+    equal_before += total >> 16;
+  }
 }
 
-// Moves the kept rows to their places.  A block takes one (sequence, head) and
-// one slice of the row's 16-byte vectors, in ascending order of the rows: row
-// j goes to a place at or before its own, so that in place a block overwrites
-// only what it has read.
-constexpr int kMoveThreads = 256;
+// Moves the kept rows to their places and their weights with them.
+//
+// To other pages, every row is free to move: a block takes a range of rows.
+// In place, row j goes to a place at or before its own, and a place may be
+// written only when what lies there has been read: a block takes a slice of
+// the rows' 16-byte vectors, all rows of it in ascending order, and writes
+// each step's rows after the whole step is read; slices are as narrow as it
+// takes to occupy the GPU.  The last block of a pair moves its weights.
+constexpr int kMoveThreads = 256, kMoveRows = 4;  // rows of a thread in a step
 
-__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(KvEvictParams p, int vecs_slice, int elem_bytes) {
+template <bool IN_PLACE>
+__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(KvEvictParams p, int vecs, int elem_bytes, int row_blocks) {
   const int kvh = blockIdx.x % p.geom.kv_heads, b = blockIdx.x / p.geom.kv_heads;
-  const int row_vecs = p.geom.head_dim * elem_bytes / 16, slices = row_vecs / vecs_slice;
-  char* pages = static_cast<char*>((int)blockIdx.y < slices ? p.k_pages : p.v_pages);
-  const int v0 = (int)blockIdx.y % slices * vecs_slice;
   const int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.y == row_blocks) {  // the weights
+    const int len = p.plan[2 * b], left = min(len, p.budget);
+    if (kvh == 0 && tid == 0) p.lengths_out[b] = p.plan[2 * b + 1];
+    const float* w = p.weights + b * p.w_batch + kvh * p.w_stride;
+    float* wo = p.weights_out + b * p.wo_batch + kvh * p.wo_stride;
+    constexpr int kEach = 8;
+    for (int j0 = 0; j0 < left; j0 += kMoveThreads * kEach) {
+      float x[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int j = j0 + e * kMoveThreads + tid;
+        x[e] = j < left ? w[kept[j]] : 0.f;
+      }
+      __syncthreads();  // read before they are written over
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int j = j0 + e * kMoveThreads + tid;
+        if (j < left) wo[j] = x[e];
+      }
+    }
+    __syncthreads();
+    for (int j = max(left, 0) + tid; j < len; j += kMoveThreads) wo[j] = 0.f;
+    return;
+  }
   const int32_t* from = p.table + b * p.table_stride;
-  const int32_t* to = p.to_table ? p.to_table + b * p.to_stride : from;
-  const int64_t to_cols = p.to_table ? p.to_cols : p.table_cols;
-  const int rows = kMoveThreads / vecs_slice;
-  if (kvh == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.lengths_out[b] = p.new_len[b];
-  for (int j0 = 0; j0 < p.budget; j0 += rows) {
-    const int j = j0 + threadIdx.x / vecs_slice;
-    int src = -1;
-    if (j < p.budget && (int)threadIdx.x < rows * vecs_slice) src = kept[j];
-    uint4 x = make_uint4(0, 0, 0, 0);
-    char* dst = nullptr;
-    if (src >= 0 && (p.to_table || src != j)) {
+  const int32_t* to = IN_PLACE ? from : p.to_table + b * p.to_stride;
+  const int64_t to_cols = IN_PLACE ? p.table_cols : p.to_cols;
+  const int row_vecs = p.geom.head_dim * elem_bytes / 16;
+  // in place: the block's slice of K or of V; else all of K's rows and all of V's
+  const int slices = row_vecs / vecs, slice = IN_PLACE ? blockIdx.y % slices : 0;
+  char* pages = static_cast<char*>(IN_PLACE && (int)blockIdx.y >= slices ? p.v_pages : p.k_pages);
+  const long long to_v = static_cast<char*>(p.v_pages) - static_cast<char*>(p.k_pages);
+  const int rows = kMoveThreads / vecs, row = tid / vecs, at = (slice * vecs + tid % vecs) * 16;
+  const int step = rows * kMoveRows;
+  const int first = IN_PLACE ? 0 : (int)blockIdx.y * step, stride = IN_PLACE ? step : row_blocks * step;
+  for (int j0 = first; j0 < p.budget; j0 += stride) {
+    uint4 x[kMoveRows], y[kMoveRows];
+    char* dst[kMoveRows];
+#pragma unroll
+    for (int r = 0; r < kMoveRows; ++r) {
+      const int j = j0 + r * rows + row;
+      dst[r] = nullptr;
+      if (row >= rows || j >= p.budget) continue;
+      const int src = kept[j];
+      if (src < 0 || (IN_PLACE && src == j)) continue;
       const int64_t fp = page_of(from, p.table_cols, src, p.geom), tp = page_of(to, to_cols, j, p.geom);
       if (fp < 0 || tp < 0) {
         set_status(p.status, ST_KV_PAGE);
-      } else {
-        const int64_t v = (int64_t)(v0 + threadIdx.x % vecs_slice) * 16;
-        x = *reinterpret_cast<const uint4*>(
-            pages + row_offset(fp, kvh, src % p.geom.page_size, p.geom) * elem_bytes + v);
-        dst = pages + row_offset(tp, kvh, j % p.geom.page_size, p.geom) * elem_bytes + v;
+        continue;
       }
+      const char* a = pages + row_offset(fp, kvh, src % p.geom.page_size, p.geom) * elem_bytes + at;
+      x[r] = *reinterpret_cast<const uint4*>(a);
+      if (!IN_PLACE) y[r] = *reinterpret_cast<const uint4*>(a + to_v);
+      dst[r] = pages + row_offset(tp, kvh, j % p.geom.page_size, p.geom) * elem_bytes + at;
     }
-    __syncthreads();  // every row of this step is read
-    if (dst) *reinterpret_cast<uint4*>(dst) = x;
+    if (IN_PLACE) __syncthreads();  // every row of this step is read
+#pragma unroll
+    for (int r = 0; r < kMoveRows; ++r)
+      if (dst[r]) {
+        *reinterpret_cast<uint4*>(dst[r]) = x[r];
+        if (!IN_PLACE) *reinterpret_cast<uint4*>(dst[r] + to_v) = y[r];
+      }
   }
 }
 
@@ -206,12 +365,26 @@ cudaError_t by_type(int dt, F f) {
   return cudaGetLastError();
 }
 
+int elem_bytes(int dt) { return dt == DT_F32 ? 4 : 2; }
+
 }  // namespace
 
 cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t s) {
   if (p.tokens == 0) return cudaSuccess;
-  const unsigned grid = (unsigned)std::min<int64_t>(p.tokens, 148 * 16);
-  return by_type(p.page_dt, [&](auto t) { kv_append_kernel<decltype(t)><<<grid, 256, 0, s>>>(p); });
+  const int vecs = p.geom.kv_heads * p.geom.head_dim * elem_bytes(p.page_dt) / 16;
+  int lanes = 1;  // threads of a token
+  while (lanes < vecs && lanes < kAppendThreads) lanes *= 2;
+  const int per_block = kAppendThreads / lanes;
+  const unsigned grid = (unsigned)((p.tokens + per_block - 1) / per_block);
+  const int es = elem_bytes(p.dt);
+  const bool aligned = reinterpret_cast<uintptr_t>(p.k) % 16 == 0 && reinterpret_cast<uintptr_t>(p.v) % 16 == 0 &&
+                       (p.tokens == 1 || (p.k_stride * es % 16 == 0 && p.v_stride * es % 16 == 0));
+  return by_type(p.page_dt, [&](auto t) {
+    by_type(p.dt, [&](auto a) {
+      if (aligned) kv_append_kernel<decltype(t), decltype(a), true><<<grid, kAppendThreads, 0, s>>>(p, lanes);
+      else kv_append_kernel<decltype(t), decltype(a), false><<<grid, kAppendThreads, 0, s>>>(p, lanes);
+    });
+  });
 }
 
 cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s) {
@@ -220,7 +393,12 @@ cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s) {
                   : p.page_dt == DT_F16 ? launch_kv_attend_f16(p, s)
                                         : launch_kv_attend_bf16(p, s);
   if (e == cudaSuccess && p.weights_out) {
-    kv_weights_kernel<<<dim3((unsigned)(p.batch * p.geom.kv_heads), 16), 256, 0, s>>>(p);
+    const int group = p.heads / p.geom.kv_heads, pairs = p.batch * p.geom.kv_heads;
+    // about eight blocks an SM over all pairs; a block beyond a sequence's end leaves at once
+    const int64_t most = (p.max_len + kWeightThreads - 1) / kWeightThreads;
+    const int64_t want = std::max<int64_t>(1, (8ll * p.sms + pairs - 1) / pairs);
+    kv_weights_kernel<<<dim3((unsigned)pairs, (unsigned)std::min<int64_t>(std::min(most, want), 65535)), kWeightThreads,
+                        sizeof(float2) * group, s>>>(p);
     e = cudaGetLastError();
   }
   return e;
@@ -228,13 +406,35 @@ cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s) {
 
 cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t s) {
   if (p.batch == 0) return cudaSuccess;
-  const unsigned pairs = (unsigned)(p.batch * p.geom.kv_heads);
-  kv_select_kernel<<<pairs, kSelectThreads, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const int es = p.page_dt == DT_F32 ? 4 : 2, row_vecs = p.geom.head_dim * es / 16;
-  const int slice = row_vecs % 2 == 0 ? 2 : 1;
-  kv_move_kernel<<<dim3(pairs, 2 * row_vecs / slice), kMoveThreads, 0, s>>>(p, slice, es);
+  const int pairs = p.batch * p.geom.kv_heads;
+  // Blocks of a pair's cluster: as many as the GPU holds at once, of 2048 positions at least.
+  int cluster = 1;
+  while (cluster < 8 && (int64_t)pairs * cluster * 2 <= 2 * p.sms && p.max_len / (cluster * 2) >= 2 * kSelectThreads)
+    cluster *= 2;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  cfg.gridDim = dim3((unsigned)(pairs * cluster));
+  cfg.blockDim = dim3(kSelectThreads);
+  cfg.stream = s;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kv_select_kernel, p)) return e;
+
+  const int es = elem_bytes(p.page_dt), row_vecs = p.geom.head_dim * es / 16;
+  if (p.to_table) {
+    const int step = kMoveThreads / row_vecs * kMoveRows;
+    const int64_t want = std::max<int64_t>(1, (16ll * p.sms + pairs - 1) / pairs);
+    const int blocks = (int)std::min<int64_t>((p.budget + step - 1) / step, std::min<int64_t>(want, 65534));
+    kv_move_kernel<false><<<dim3((unsigned)pairs, (unsigned)blocks + 1), kMoveThreads, 0, s>>>(p, row_vecs, es, blocks);
+  } else {
+    int vecs = row_vecs;  // of a slice: halved while the slices leave SMs idle
+    while (vecs % 2 == 0 && (int64_t)pairs * 2 * (row_vecs / vecs) < 8ll * p.sms) vecs /= 2;
+    const int slices = row_vecs / vecs;
+    kv_move_kernel<true><<<dim3((unsigned)pairs, (unsigned)(2 * slices + 1)), kMoveThreads, 0, s>>>(p, vecs, es, 2 * slices);
+  }
   return cudaGetLastError();
 }
 

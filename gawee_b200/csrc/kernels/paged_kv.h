@@ -85,7 +85,8 @@ struct KvEvictParams {
   int64_t max_len;
   int batch, budget, recent;
   int32_t* kept;     // [batch][kv_heads][budget]
-  int32_t* new_len;  // [batch] scratch
+  int32_t* plan;     // [batch][2] scratch: rows before, and the length to pass on
+  int sms;
   int* status;
 };
 cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t s);
