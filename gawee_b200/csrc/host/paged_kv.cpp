@@ -171,7 +171,7 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device);
     const size_t parts = (size_t)2 * kv->sms * kKvMaxBlocksPerSm;
     const int block_heads = d.heads / d.kv_heads > 8 ? kKvHeadsMost : 8;
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->parts, sizeof(float) * parts * block_heads * (d.head_dim + 2));
+    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->parts, sizeof(float) * parts * (block_heads * (d.head_dim + 2) + 4));
     if (e == cudaSuccess) e = cudaMalloc((void**)&kv->arrived, sizeof(unsigned) * 2 * parts);
     if (e == cudaSuccess) e = cudaMemset(kv->arrived, 0, sizeof(unsigned) * 2 * parts);
     if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));

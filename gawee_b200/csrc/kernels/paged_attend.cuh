@@ -89,6 +89,13 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ void add_scaled(float4& to, const float4& x, float f) {
+  to.x += x.x * f;
+  to.y += x.y * f;
+  to.z += x.z * f;
+  to.w += x.w * f;
+}
+
 // --- the two ways to compute a tile ---------------------------------------------
 //
 // Lanes: any types.  L lanes hold a key's row, eight elements each (D <= 8 L),
@@ -114,6 +121,7 @@ struct LaneTile {
   // pairs, then a factor a head; in units of 16 bytes.
   static constexpr int kScratch = 2 * TK * NH + (NH + 3) / 4 * 4;
   static constexpr int kD = FULL ? 8 * L : 0;
+  static constexpr int kMinBlocks = NH <= 4 ? 3 : 2;  // of an SM: what the stages leave room for
   static_assert(2 * TK * sizeof(T) >= NH * 4, "a warp's state fits into a stage");
 
   uint64_t q[NH][4], acc[NH][4];
@@ -343,6 +351,7 @@ struct MmaTile {
   static constexpr int kScratch = 0;
   static constexpr int kD = FULL ? DT : 0;
   static constexpr int R = NH / 8;  // head rows of a thread
+  static constexpr int kMinBlocks = DT == 256 ? 1 : 2;
   static_assert(2 * TK * DT * 2 >= NH * DT * 4, "a warp's state fits into a stage");
 
   uint32_t q[DT / 16][2 * R];
@@ -573,7 +582,7 @@ constexpr int kMostParts = 32;
 static_assert(kMostParts * kMostParts >= kKvMaxBlocksPerSm * 256, "two levels cover the grid");
 
 template <class P>
-__global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_constant__ KvAttendParams p) {
+__global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(const __grid_constant__ KvAttendParams p) {
   using T = typename P::T;
   constexpr int TK = P::TK, TILE = kWarps * TK, NS = P::kStages, NH = P::NH;
   extern __shared__ __align__(128) char smem[];
@@ -795,100 +804,120 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
     copy_commit();
   }
 
-  P state;
   int stage = 0, load_stage = NS - 1;  // of the tile in use, and of the next tile to load
-  bool fresh_segment = true;
   long long seg_begin = t0 - use.tile;  // the segment's first tile
+  int j = 0;
 #pragma unroll 1
-  for (int j = 0; j < count; ++j) {
+  while (j < count) {  // a segment, or the part of it that this block has
     const int h0 = use.kvh * group + use.chunk * NH, nh = min(NH, group - use.chunk * NH);
-    if (fresh_segment) state.begin(p, use.b, h0, nh);
-    fresh_segment = false;
-    copy_wait<NS - 2>();
-    __syncwarp();
-    if (issued < count) {
-      issue(load, load_stage);
-      if (++issued < count) {
-        advance(load);
-        fetch(load);
+    const int mine = min(use.tiles - use.tile, count - j);
+    const bool seg_end = use.tile + mine == use.tiles;
+    int stage_at = 0;
+    {
+      P state;
+      state.begin(p, use.b, h0, nh);
+      int first = use.tile * TILE + warp * TK;
+      float* scores = nullptr;
+      if (p.weights_out)
+        scores = p.scores + (((long long)use.b * kv + use.kvh) * p.max_len + first) * group + use.chunk * NH;
+#pragma unroll 1
+      for (int i = 0; i < mine; ++i) {
+        copy_wait<NS - 2>();
+        __syncwarp();
+        if (issued < count) {
+          issue(load, load_stage);
+          if (++issued < count) {
+            advance(load);
+            fetch(load);
+          }
+        }
+        copy_commit();
+        load_stage = load_stage + 1 == NS ? 0 : load_stage + 1;
+        stage_at = stage * stage_bytes;
+        if (first < use.len)
+          state.tile(ring + stage_at, ring + stage_at + TK * rb, adds + stage * TK, scratch, scores, use.len - first, group,
+                     nh);
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        first += TILE;
+        if (p.weights_out) scores += (long long)TILE * group;
       }
-    }
-    copy_commit();
-    load_stage = load_stage + 1 == NS ? 0 : load_stage + 1;
-    const int first = use.tile * TILE + warp * TK;
-    if (first < use.len) {
-      float* scores = p.weights_out
-                          ? p.scores + (((long long)use.b * kv + use.kvh) * p.max_len + first) * group + use.chunk * NH
-                          : nullptr;
-      state.tile(ring + stage * stage_bytes, ring + stage * stage_bytes + TK * rb, adds + stage * TK, scratch, scores,
-                 use.len - first, group, nh);
-    }
-    const bool seg_end = use.tile + 1 == use.tiles;
-    if (seg_end || j + 1 == count) {
-      // join the warps
-      const int stage_at = stage * stage_bytes;
+      // the warp's state takes the place of the stage it has just used
       state.dump(&s_ml[warp][0][0], reinterpret_cast<float*>(ring + stage_at));
+    }
+    j += mine;
+    use.tile += mine - 1;  // its last tile here
+    {
+      // join the warps
       __syncthreads();
       const long long seg_last = seg_begin + use.tiles - 1;
       const bool whole = seg_begin >= t0 && seg_end;
-      auto part_at = [&](long long slot) { return p.parts + slot * NH * (D + 2); };  // [NH][2], then [nh][D]
-      auto finish = [&](int x, float mt, float lt, float ot) {
-        const int h = x / D, d = x % D;
-        store_act(p.out, p.dt, use.b * p.out_stride + (int64_t)h0 * D + x, lt != 0.f ? ot / lt : 0.f);
+      // A part in the workspace: [NH][2], padded to 16 bytes, then [nh][D], counted
+      // in units of 16 bytes.  A block has two places: 2 i + 1 for the segment that begins
+      // in its run and goes on behind it, 2 i for the one that began before.
+      constexpr int kHead4 = (2 * NH + 3) / 4;
+      const int part4 = NH * D / 4 + kHead4;
+      float4* parts = reinterpret_cast<float4*>(p.parts);
+      const int dv = D / 4;  // the results are taken four at a time
+      auto finish = [&](int x, float mt, float lt, const float4& o) {
+        const int h = x / dv, d = x % dv * 4;
+        const int64_t at = use.b * p.out_stride + (int64_t)(h0 + h) * D + d;
+        const bool any = lt != 0.f;
+        store_act4(p.out, p.dt, at, any ? o.x / lt : 0.f, any ? o.y / lt : 0.f, any ? o.z / lt : 0.f, any ? o.w / lt : 0.f);
         if (p.weights_out && d == 0) {
           p.stats[((int64_t)use.b * p.heads + h0 + h) * 2] = mt;
           p.stats[((int64_t)use.b * p.heads + h0 + h) * 2 + 1] = lt;
         }
       };
-      long long slot = 2ll * blockIdx.x + (seg_begin <= t0 ? 0 : 1);
-      for (int x = tid; x < nh * D; x += kThreads) {
-        const int h = x / D;
-        float mt = -INFINITY, lt = 0.f, ot = 0.f;
+      auto leave = [&](int place, int x, float mt, float lt, const float4& o) {
+        float4* q = parts + place * part4;
+        q[kHead4 + x] = o;
+        if (x % dv == 0) reinterpret_cast<float2*>(q)[x / dv] = make_float2(mt, lt);
+      };
+      const int own_place = 2 * blockIdx.x + (seg_begin >= t0 ? 1 : 0);
+      for (int x = tid; x < nh * dv; x += kThreads) {
+        const int h = x / dv;
+        float mt = -INFINITY, lt = 0.f;
+        float4 ot = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, s_ml[w][h][0]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float c = exp_from(s_ml[w][h][0], mt);
           lt += s_ml[w][h][1] * c;
-          ot += reinterpret_cast<const float*>(smem + w * NS * stage_bytes + stage_at)[x] * c;
+          add_scaled(ot, reinterpret_cast<const float4*>(smem + w * NS * stage_bytes + stage_at)[x], c);
         }
-        if (whole) {
-          finish(x, mt, lt, ot);
-        } else {
-          part_at(slot)[2 * NH + x] = ot;
-          if (x % D == 0) {
-            part_at(slot)[2 * h] = mt;
-            part_at(slot)[2 * h + 1] = lt;
-          }
-        }
+        if (whole) finish(x, mt, lt, ot);
+        else leave(own_place, x, mt, lt, ot);
       }
       if (!whole) {
         // The segment's blocks are c0 .. c1; the one that holds tile t is the
-        // largest i with floor(total * i / blocks) <= t.  Block c left its part in its slot 0, or
-        // c0, where an earlier segment took that, in slot 1.
+        // largest i with floor(total * i / blocks) <= t.
         const int c0 = (int)(((seg_begin + 1) * blocks - 1) / total);
         const int n = (int)(((seg_last + 1) * blocks - 1) / total) - c0 + 1;
-        const long long base = 2ll * c0, first_slot = base + (total * c0 / blocks >= seg_begin ? 0 : 1);
-        int fan = 8;  // parts of a group
-        while (fan * fan < n) fan *= 2;
+        auto place_of = [&](int i) { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
+        int fan = kMostParts;  // parts of a group
+        if (n > kMostParts)
+          for (fan = 8; fan * fan < n;) fan *= 2;
         const int me = blockIdx.x - c0;
         for (int level = 0, step = 1; level < 2; ++level, step = fan) {
           // this block's group: parts lo, lo + step, .. below hi; it is complete with its last arrival
           const int lo = level == 0 ? me / fan * fan : 0, hi = level == 0 ? min(lo + fan, n) : n;
           const int k = (hi - lo + step - 1) / step;
           if (level == 1 && n <= fan) break;
-          auto slot_of = [&](int i) { return i == 0 ? first_slot : base + 2ll * i; };
-          __threadfence();
           __syncthreads();
-          if (tid == 0)  // the counter wraps to 0 with the last arrival: ready for the next call
-            s_last = k == 1 || atomicInc(p.arrived + 2 * slot_of(lo) + level, k - 1) == (unsigned)(k - 1);
+          if (tid == 0) {
+            // the fences are cumulative over the block's barriers; the counter wraps to
+            // 0 with the last arrival: ready for the next call
+            __threadfence();
+            s_last = k == 1 || atomicInc(p.arrived + 2 * place_of(lo) + level, k - 1) == (unsigned)(k - 1);
+            __threadfence();
+          }
           __syncthreads();
           if (!s_last) break;
-          __threadfence();
           if (k == 1) continue;
           for (int h = warp; h < nh; h += kWarps) {
-            const float* q = part_at(slot_of(lo + min(lane, k - 1) * step));
-            const float m = lane < k ? __ldcg(q + 2 * h) : -INFINITY, l = lane < k ? __ldcg(q + 2 * h + 1) : 0.f;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + place_of(lo + min(lane, k - 1) * step) * part4) + h);
+            const float m = lane < k ? ml.x : -INFINITY, l = lane < k ? ml.y : 0.f;
             float mt = m;
 #pragma unroll
             for (int o = 16; o; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
@@ -896,7 +925,7 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
             float lt = l * f;
 #pragma unroll
             for (int o = 16; o; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
-            s_part[lane][h] = f;
+            s_part[lane][h] = f;  // 0 behind the last part
             if (lane == 0) {
               s_top[h][0] = mt;
               s_top[h][1] = lt;
@@ -904,30 +933,31 @@ __global__ void __launch_bounds__(kThreads) kv_attend_kernel(const __grid_consta
           }
           __syncthreads();
           const bool done = level == 1 || n <= fan;
-          for (int x = tid; x < nh * D; x += kThreads) {
-            const int h = x / D;
-            float ot = 0.f;
-#pragma unroll 8
-            for (int i = 0; i < k; ++i) ot += __ldcg(part_at(slot_of(lo + i * step)) + 2 * NH + x) * s_part[i][h];
-            if (done) {
-              finish(x, s_top[h][0], s_top[h][1], ot);
-            } else {  // in place of the group's first part, which no other block reads any more
-              part_at(slot_of(lo))[2 * NH + x] = ot;
-              if (x % D == 0) {
-                part_at(slot_of(lo))[2 * h] = s_top[h][0];
-                part_at(slot_of(lo))[2 * h + 1] = s_top[h][1];
-              }
+          for (int x = tid; x < nh * dv; x += kThreads) {
+            const int h = x / dv;
+            float4 ot = make_float4(0, 0, 0, 0);
+            const float4* q = parts + kHead4 + x;
+            const int first_place = place_of(lo), stride = 2 * step * part4;
+            int at = 2 * (c0 + lo) * part4;
+            for (int i0 = 0; i0 < k; i0 += 8, at += 8 * stride) {  // eight loads on the way
+              float4 o[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (i0 + i < k) o[i] = __ldcg(q + (i0 + i == 0 ? first_place * part4 : at + i * stride));
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (i0 + i < k) add_scaled(ot, o[i], s_part[i0 + i][h]);
             }
+            if (done) finish(x, s_top[h][0], s_top[h][1], ot);
+            else leave(first_place, x, s_top[h][0], s_top[h][1], ot);  // no other block reads that part any more
           }
         }
       }
       __syncthreads();  // the stages are free again
       if (padded) clear(ring + stage_at, stage_bytes);
-      if (j + 1 < count) seg_begin = seg_last + 1;
-      fresh_segment = true;
+      seg_begin = seg_last + 1;
     }
-    if (j + 1 < count) advance(use);
-    stage = stage + 1 == NS ? 0 : stage + 1;
+    if (j < count) advance(use);
   }
   copy_wait<0>();
   if (blockIdx.x == 0)  // lengths that length_of took as 0

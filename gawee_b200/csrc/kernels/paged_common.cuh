@@ -46,10 +46,18 @@ __device__ __forceinline__ float load_act(const void* p, int dt, int64_t i) {
   if (dt == DT_F16) return to_f(static_cast<const __half*>(p)[i]);
   return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
 }
-__device__ __forceinline__ void store_act(void* p, int dt, int64_t i, float x) {
-  if (dt == DT_F32) static_cast<float*>(p)[i] = x;
-  else if (dt == DT_F16) static_cast<__half*>(p)[i] = from_f<__half>(x);
-  else static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(x);
+
+template <class A>
+__device__ __forceinline__ void store4(A* p, float a, float b, float c, float d) {
+  p[0] = from_f<A>(a);
+  p[1] = from_f<A>(b);
+  p[2] = from_f<A>(c);
+  p[3] = from_f<A>(d);
+}
+__device__ __forceinline__ void store_act4(void* p, int dt, int64_t i, float a, float b, float c, float d) {
+  if (dt == DT_F32) store4(static_cast<float*>(p) + i, a, b, c, d);
+  else if (dt == DT_F16) store4(static_cast<__half*>(p) + i, a, b, c, d);
+  else store4(static_cast<__nv_bfloat16*>(p) + i, a, b, c, d);
 }
 
 }  // namespace paged
