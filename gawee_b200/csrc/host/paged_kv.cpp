@@ -37,8 +37,6 @@ struct gawee_kv {
 
 namespace {
 
-using gawee::kern::kKvHeadsMost;
-using gawee::kern::kKvMaxBlocksPerSm;
 using gawee::kern::PageGeom;
 
 gawee_status fail(gawee_status st, const std::string& what) {
@@ -169,11 +167,12 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     if (e == cudaSuccess && d.weights)
       e = cudaMalloc((void**)&kv->scores, sizeof(float) * rows * d.max_pages * d.page_size);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device);
-    const size_t parts = (size_t)2 * kv->sms * kKvMaxBlocksPerSm;
-    const int block_heads = d.heads / d.kv_heads > 8 ? kKvHeadsMost : 8;
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->parts, sizeof(float) * parts * (block_heads * (d.head_dim + 2) + 4));
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->arrived, sizeof(unsigned) * 2 * parts);
-    if (e == cudaSuccess) e = cudaMemset(kv->arrived, 0, sizeof(unsigned) * 2 * parts);
+    if (e == cudaSuccess)
+      e = cudaMalloc((void**)&kv->parts,
+                     sizeof(float) * gawee::kern::kv_parts_floats(kv->sms, d.heads / d.kv_heads, d.head_dim));
+    const size_t counters = sizeof(unsigned) * gawee::kern::kv_counters(kv->sms);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->arrived, counters);
+    if (e == cudaSuccess) e = cudaMemset(kv->arrived, 0, counters);
     if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
@@ -313,9 +312,7 @@ gawee_status gawee_kv_attend(gawee_kv* kv, const gawee_kv_attend_args* a, void* 
     p.arrived = kv->arrived;
     p.device = kv->device;
     p.sms = kv->sms;
-    p.page_shift = -1;
-    for (int b = 0; b <= 16; ++b)
-      if (kv->geom.page_size == 1 << b) p.page_shift = b;
+    p.page_shift = gawee::kern::page_shift_of(kv->geom.page_size);
     p.status = kv->status;
     return run_on(kv, kName, [&] { return launch_kv_attend(p, static_cast<cudaStream_t>(stream)); });
   });

@@ -13,6 +13,7 @@
 #include <stdexcept>
 
 #include "../kernels/kernels.h"
+#include "../kernels/paged_kv.h"
 #include "launch.h"
 
 namespace gawee {
@@ -170,6 +171,7 @@ class Planner {
         v = copy_to_new(v, "result_copy");
       plan_->result_view.push_back(v);
     }
+    check_pages();
     assign_phases();
     fuse_elementwise();
     fuse_epilogues();
@@ -182,6 +184,8 @@ class Planner {
  private:
   std::unique_ptr<Plan> plan_;
   std::vector<bool> has_view_;
+  std::set<int> page_bufs_;  // the pages arguments of paged_attention ops
+  int kv_counters_ = -1;     // their arrival counters' buffer
 
   // ---------------------------------------------------------------- attention clusters
   // matmul(Q, KT) -> div(A, c) [-> add(., mask)] -> softmax(-1) -> matmul(P, V),
@@ -963,6 +967,7 @@ class Planner {
     if (k == "shape") return plan_shape(n);
     if (k == "tile" || k == "pad" || k == "resize") return plan_remap(n, k);
     if (k == "topk") return plan_topk(n);
+    if (k == "paged_attention") return plan_paged_attention(n);
     unsupported("gawee op " + k);
   }
 
@@ -1854,6 +1859,77 @@ class Planner {
     add_op(std::move(op));
     set_view(n.outs[0], vals);
     set_view(n.outs[1], idxs);
+  }
+
+  // gawee.paged_attention(q, k, v, k_pages, v_pages, block_table, lengths): one
+  // decode step over a paged key/value cache (include/gawee_cuda.h,
+  // gawee_kv_attend).  The pages are two arguments of their own: the op stores the new rows
+  // there, in place, and they keep them from one forward to the next.  Not a
+  // reference op: its decode step concatenates the cache (CatOpLowering).
+  void plan_paged_attention(const Node& n) {
+    if (n.ins.size() != 7) unsupported("paged_attention takes 7 operands");
+    auto rows = [&](int value, const char* what) {  // [B, heads, D], each row dense
+      View v = value_view(value);
+      if (v.rank() != 3 || v.dt != DType::F32) unsupported(std::string("paged_attention: ") + what + " must be f32 [B, heads, D]");
+      if (v.st[2] != 1 || (v.shape[1] > 1 && v.st[1] != v.shape[2])) v = copy_to_new(v, "paged_attention_copy");
+      return v;
+    };
+    View q = rows(n.ins[0], "q"), k = rows(n.ins[1], "k"), v = rows(n.ins[2], "v");
+    View pages[2];
+    for (int i = 0; i < 2; ++i) {
+      pages[i] = value_view(n.ins[3 + i]);
+      const View& p = pages[i];
+      if (p.rank() != 4 || p.dt != DType::F32 || plan_->bufs[p.buf].kind != BufKind::ARG || !p.dense_rowmajor() ||
+          p.numel() != plan_->bufs[p.buf].elems)
+        unsupported("paged_attention: the pages must be function arguments f32 [pages, kv_heads, page_size, D]");
+      if (!page_bufs_.insert(p.buf).second) unsupported("paged_attention: a pages argument used twice");
+    }
+    View table = value_view(n.ins[5]), lengths = value_view(n.ins[6]);
+    const int64_t B = q.shape[0], H = q.shape[1], D = q.shape[2], KV = k.shape[1];
+    if (table.rank() != 2 || table.dt != DType::I32 || table.shape[0] != B || table.shape[1] < 1)
+      unsupported("paged_attention: block_table must be i32 [B, columns]");
+    if (lengths.rank() != 1 || lengths.dt != DType::I32 || lengths.shape[0] != B)
+      unsupported("paged_attention: lengths must be i32 [B]");
+    if (!table.dense_rowmajor()) table = copy_to_new(table, "paged_attention_copy");
+    if (!lengths.dense_rowmajor()) lengths = copy_to_new(lengths, "paged_attention_copy");
+    if (k.shape != v.shape || k.shape[0] != B || k.shape[2] != D || KV < 1 || H % KV)
+      unsupported("paged_attention: k and v must be [B, kv_heads, D], heads a multiple of kv_heads");
+    const auto& ps = pages[0].shape;
+    if (pages[1].shape != ps || ps[1] != KV || ps[3] != D || ps[2] < 1 || ps[2] > 65536)
+      unsupported("paged_attention: the pages' shape does not match k and v");
+    if (D < 8 || D > 256 || D % 8) unsupported("paged_attention: D must be a multiple of 8 up to 256");
+    if (B > 65535 || H > 65535 || ps[0] > INT32_MAX || table.shape[1] * ps[2] > INT32_MAX - (1 << 20))
+      unsupported("paged_attention: batch, heads, pages or rows beyond the limits of gawee_kv_create");
+    const Attr& sc = n.attr("scale");
+    const double scale = sc.kind == Attr::INT ? (double)sc.i : sc.f;
+    View out = alloc(DType::F32, val(n.outs[0]).type.shape);
+    if (out.shape != q.shape) unsupported("paged_attention: the result has q's shape");
+    View parts = alloc(DType::F32, {kern::kv_parts_floats(kern::kKvPlanSms, (int)(H / KV), (int)D)});
+    // counters that are 0 between calls; the calls of a forward follow one another, so one set serves them all
+    if (kv_counters_ < 0) {
+      kv_counters_ = new_buf(DType::I32, kern::kv_counters(kern::kKvPlanSms), BufKind::CONST);
+      plan_->bufs[kv_counters_].host_init.assign(4 * (size_t)kern::kv_counters(kern::kKvPlanSms), 0);
+    }
+    View arrived = dense_view(kv_counters_, DType::I32, {kern::kv_counters(kern::kKvPlanSms)});
+    Op op;
+    op.kind = OpKind::PAGED_ATTN;
+    op.name = "paged_attention";
+    op.reads = {q, k, v, pages[0], pages[1], table, lengths, arrived};
+    op.writes = {out, parts};
+    op.launch = launch::paged_attention(q, k, v, pages[0], pages[1], table, lengths, out, parts, arrived, (float)scale);
+    add_op(std::move(op));
+    set_view(n.outs[0], out);
+  }
+
+  // A pages argument is state that its one op reads and writes in place.
+  void check_pages() {
+    std::map<int, int> used;
+    for (const Op& op : plan_->ops)
+      if (!op.dead)
+        for (const View& r : op.reads)
+          if (page_bufs_.count(r.buf)) ++used[r.buf];
+    for (const auto& u : used)
+      if (u.second != 1) unsupported("a pages argument of paged_attention is used elsewhere too");
   }
 
   // The tensor-core kernel gathers A with 16-byte loads: every stepped A

@@ -58,7 +58,7 @@ struct Buf {
   size_t bytes() const { return (size_t)elems * dtype_size(dt); }
 };
 
-enum class OpKind { EW, REDUCE, GREDUCE, SOFTMAX, GATHER, GATHER_ELEMS, REMAP, RANGE, POOL, TOPK, PACK, TC, ATTN };
+enum class OpKind { EW, REDUCE, GREDUCE, SOFTMAX, GATHER, GATHER_ELEMS, REMAP, RANGE, POOL, TOPK, PACK, TC, ATTN, PAGED_ATTN };
 
 struct Runtime;  // execution state (device pointers), runtime.cpp
 

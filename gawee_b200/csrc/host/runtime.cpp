@@ -20,6 +20,7 @@
 
 #include "../../../include/gawee_cuda.h"
 #include "../kernels/kernels.h"
+#include "../kernels/paged_kv.h"
 #include "ir.h"
 #include "launch.h"
 #include "plan.h"
@@ -1023,6 +1024,42 @@ Fn topk(const View& in, const View& vals, const View& idxs, const View& used, in
   };
 }
 
+Fn paged_attention(const View& q, const View& k, const View& v, const View& k_pages, const View& v_pages,
+                   const View& table, const View& lengths, const View& out, const View& parts, const View& arrived,
+                   float scale) {
+  kern::KvAttendParams p{};
+  const auto& ps = k_pages.shape;
+  p.geom = kern::PageGeom{ps[1] * ps[2] * ps[3], ps[0], (int)ps[1], (int)ps[2], (int)ps[3]};
+  p.page_dt = p.dt = kern::DT_F32;
+  p.q_stride = q.st[0];
+  p.out_stride = out.st[0];
+  p.k_stride = k.st[0];
+  p.v_stride = v.st[0];
+  p.batch = (int)q.shape[0];
+  p.heads = (int)q.shape[1];
+  p.scale = scale;
+  p.table_stride = p.table_cols = table.shape[1];
+  p.max_len = table.shape[1] * ps[2];
+  p.page_shift = kern::page_shift_of((int)ps[2]);
+  return [=](Runtime& rt, void* s) mutable {
+    p.q = rt.ptr(q);
+    p.k = rt.ptr(k);
+    p.v = rt.ptr(v);
+    p.k_pages = rt.ptr(k_pages);
+    p.v_pages = rt.ptr(v_pages);
+    p.table = reinterpret_cast<const int32_t*>(rt.ptr(table));
+    p.lengths = reinterpret_cast<const int32_t*>(rt.ptr(lengths));
+    p.out = rt.ptr(out);
+    p.parts = reinterpret_cast<float*>(rt.ptr(parts));
+    p.arrived = reinterpret_cast<unsigned*>(rt.ptr(arrived));
+    p.status = rt.status();
+    p.device = rt.device;
+    if (!p.sms) GCHECK(cudaDeviceGetAttribute(&p.sms, cudaDevAttrMultiProcessorCount, rt.device));
+    p.sms = std::min(p.sms, kern::kKvPlanSms);
+    GCHECK(kern::launch_kv_attend(p, static_cast<cudaStream_t>(s)));
+  };
+}
+
 Fn pack(const PackSpec& ps, int64_t ldk, int hi, int lo) {
   kern::PackBParams pp{};
   pp.batch = ps.batch;
@@ -1228,6 +1265,18 @@ gawee_status gawee_set_arg(gawee_ctx* ctx, int i, const void* host, size_t bytes
 
 gawee_status gawee_set_arg_device(gawee_ctx* ctx, int i, const void* dev, size_t bytes, void* stream) {
   return set_arg_impl(ctx, i, dev, bytes, stream, cudaMemcpyDeviceToDevice);
+}
+
+gawee_status gawee_arg_device_ptr(gawee_ctx* ctx, int i, void** ptr) {
+  if (!ctx || !ptr) return GAWEE_ERR_INVALID;
+  *ptr = nullptr;
+  return guard(ctx, [&] {
+    auto& rt = ctx->rt;
+    if (i < 0 || i >= (int)rt.plan->arg_buf.size()) throw gawee::StatusError(GAWEE_ERR_INVALID, "argument index out of range");
+    const gawee::Buf& b = rt.plan->bufs[rt.plan->arg_buf[i]];
+    if (!b.ptr) throw gawee::StatusError(GAWEE_ERR_INVALID, "argument " + std::to_string(i) + " has no device memory");
+    *ptr = b.ptr;
+  });
 }
 
 gawee_status gawee_forward(gawee_ctx* ctx, void* stream) {

@@ -21,6 +21,13 @@ struct PageGeom {
   int kv_heads, page_size, head_dim;
 };
 
+// log2 of a page size, -1 where it is no power of two.
+inline int page_shift_of(int page_size) {
+  for (int b = 0; b <= 16; ++b)
+    if (page_size == 1 << b) return b;
+  return -1;
+}
+
 // The page that holds row `pos` of the sequence whose block-table row is
 // `table` (`cols` columns), or -1 where the table has no such column or names
 // a page that does not exist.

@@ -15,6 +15,15 @@ namespace kern {
 // that an SM holds at most.  They size the workspace.
 constexpr int kKvHeadsMost = 16, kKvMaxBlocksPerSm = 4;
 
+// The attention's workspace on `sms` SMs: floats of the partial states, and
+// counters, 0 before the first call (every call leaves them 0).
+inline int64_t kv_parts_floats(int sms, int group, int head_dim) {
+  return (int64_t)2 * sms * kKvMaxBlocksPerSm * ((group > 8 ? kKvHeadsMost : 8) * (head_dim + 2) + 4);
+}
+inline int64_t kv_counters(int sms) { return (int64_t)4 * sms * kKvMaxBlocksPerSm; }
+// SMs that a graph's workspace is planned for; a GPU with more uses this many.
+constexpr int kKvPlanSms = 160;
+
 // Rows of new tokens into the pages: token t's key k[t * k_stride + h * D ..]
 // goes to row positions[t] of sequence sequences[t] (nullptr: sequence t).  A
 // token with a negative position or sequence is left out.

@@ -23,6 +23,7 @@ None: the device's default stream).  Errors that only the device can see
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 from .runtime import GaweeError, _stream_ptr, load_library
@@ -31,35 +32,11 @@ DTYPES = {"f32": 0, "f16": 2, "bf16": 7}
 _NAMES = {"float32": 0, "float16": 2, "bfloat16": 7, "int32": 4}
 _dtype_codes: dict = {}
 
-_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
-
-
-class _Desc(ctypes.Structure):
-    _fields_ = [("dtype", _I), ("heads", _I), ("kv_heads", _I), ("head_dim", _I), ("page_size", _I),
-                ("num_pages", _L), ("page_stride", _L), ("max_batch", _I), ("max_pages", _I), ("weights", _I)]
-
-
-class _Append(ctypes.Structure):
-    _fields_ = [("k_pages", _P), ("v_pages", _P), ("k", _P), ("v", _P), ("dtype", _I), ("k_stride", _L),
-                ("v_stride", _L), ("tokens", _L), ("sequences", _P), ("positions", _P), ("block_table", _P),
-                ("table_stride", _L), ("table_cols", _I), ("batch", _I)]
-
-
-class _Attend(ctypes.Structure):
-    _fields_ = [("k_pages", _P), ("v_pages", _P), ("q", _P), ("out", _P), ("dtype", _I), ("q_stride", _L),
-                ("out_stride", _L), ("batch", _I), ("scale", _F), ("block_table", _P), ("table_stride", _L),
-                ("table_cols", _I), ("lengths", _P), ("k", _P), ("v", _P), ("k_stride", _L), ("v_stride", _L),
-                ("mask", _P), ("mask_stride", _L), ("mask_cols", _L), ("weights", _P), ("weights_stride", _L),
-                ("weights_batch_stride", _L), ("weights_out", _P), ("weights_out_stride", _L),
-                ("weights_out_batch_stride", _L), ("weights_cols", _L)]
-
-
-class _Evict(ctypes.Structure):
-    _fields_ = [("k_pages", _P), ("v_pages", _P), ("weights", _P), ("weights_stride", _L),
-                ("weights_batch_stride", _L), ("weights_out", _P), ("weights_out_stride", _L),
-                ("weights_out_batch_stride", _L), ("weights_cols", _L), ("batch", _I), ("block_table", _P),
-                ("table_stride", _L), ("table_cols", _I), ("to_table", _P), ("to_stride", _L), ("to_cols", _I),
-                ("lengths", _P), ("lengths_out", _P), ("budget", _I), ("recent", _I), ("kept", _P)]
+# The argument structures of include/gawee_cuda.h, packed with C alignment.
+_DESC = struct.Struct("@iiiiiqqiii")
+_APPEND = struct.Struct("@PPPPiqqqPPPqii")
+_ATTEND = struct.Struct("@PPPPiqqifPqiPPPqqPqqPqqPqqq")
+_EVICT = struct.Struct("@PPPqqPqqqiPqiPqiPPiiP")
 
 
 def _code(t) -> int:
@@ -98,15 +75,19 @@ class PagedKV:
                 raise _invalid(f"{name} is {n}")
         self._lib = load_library()
         h = ctypes.c_void_p()
-        desc = _Desc(DTYPES[dtype], heads, kv_heads, head_dim, page_size, num_pages, page_stride, max_batch,
-                     max_pages, 1 if weights else 0)
-        self._check(self._lib.gawee_kv_create(ctypes.byref(desc), device, ctypes.byref(h)))
+        try:
+            desc = _DESC.pack(DTYPES[dtype], heads, kv_heads, head_dim, page_size, num_pages, page_stride, max_batch,
+                              max_pages, 1 if weights else 0)
+        except struct.error as e:
+            raise _invalid(str(e)) from None
+        self._check(self._lib.gawee_kv_create(desc, device, ctypes.byref(h)))
         self._h = h
         self.device = device
         self._dt = DTYPES[dtype]
         self.heads, self.kv_heads, self.head_dim, self.page_size = heads, kv_heads, head_dim, page_size
         self._page_shape = (num_pages, kv_heads, page_size, head_dim)
         self._page_stride = page_stride or kv_heads * page_size * head_dim
+        self._page_strides = (self._page_stride, page_size * head_dim, head_dim, 1)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -130,24 +111,26 @@ class PagedKV:
         """The address of `t`, of dtype `code` (None: f32, f16 or bf16) on the handle's device."""
         if t.get_device() != self.device:
             raise _invalid(f"{name} is on device {t.get_device()}, the handle on {self.device}")
-        c = _code(t)
+        c = _dtype_codes.get(t.dtype)
+        if c is None:
+            c = _code(t)
         if c != code if code is not None else c not in (0, 2, 7):
             raise _invalid(f"{name} has dtype {t.dtype}")
         return t.data_ptr()
 
     def _pages(self, t, name: str) -> int:
-        if tuple(t.shape) != self._page_shape:
+        if t.shape != self._page_shape:
             raise _invalid(f"{name} has shape {tuple(t.shape)}, expected {self._page_shape}")
-        n, kvh, page, dim = self._page_shape
         s = t.stride()
-        if (s[3] != 1 or (page > 1 and s[2] != dim) or (kvh > 1 and s[1] != page * dim)
+        n, kvh, page, dim = self._page_shape
+        if s != self._page_strides and (s[3] != 1 or (page > 1 and s[2] != dim) or (kvh > 1 and s[1] != page * dim)
                 or (n > 1 and s[0] != self._page_stride)):
             raise _invalid(f"{name} has strides {tuple(s)}: pages are dense, {self._page_stride} elements apart")
         return self._on_device(t, name, self._dt)
 
     def _rows(self, t, name: str, n: int, heads: int, code: Optional[int]):
         """(address, stride between rows) of [n, heads, head_dim] with dense rows."""
-        if tuple(t.shape) != (n, heads, self.head_dim):
+        if t.shape != (n, heads, self.head_dim):
             raise _invalid(f"{name} has shape {tuple(t.shape)}, expected {(n, heads, self.head_dim)}")
         s = t.stride()
         if s[2] != 1 or (heads > 1 and s[1] != self.head_dim):
@@ -155,19 +138,20 @@ class PagedKV:
         return self._on_device(t, name, code), s[0]
 
     def _ints(self, t, name: str, n: int) -> int:
-        if tuple(t.shape) != (n,) or (n > 1 and t.stride()[0] != 1):
+        if t.shape != (n,) or (n > 1 and t.stride()[0] != 1):
             raise _invalid(f"{name} must be a dense array of {n} int32 values, got shape {tuple(t.shape)}")
         return self._on_device(t, name, 4)
 
     def _table(self, t, name: str):
         """(address, stride, rows, columns)"""
-        if len(t.shape) != 2 or (t.shape[1] > 1 and t.stride()[1] != 1):
+        shape, s = t.shape, t.stride()
+        if len(shape) != 2 or (shape[1] > 1 and s[1] != 1):
             raise _invalid(f"{name} must be int32 [batch, columns] with dense rows")
-        return self._on_device(t, name, 4), t.stride()[0], t.shape[0], t.shape[1]
+        return self._on_device(t, name, 4), s[0], shape[0], shape[1]
 
     def _weights(self, t, name: str, batch: int):
         """(address, stride between heads, between sequences, columns)"""
-        if len(t.shape) != 3 or tuple(t.shape[:2]) != (batch, self.kv_heads) or t.shape[2] < 1 or t.stride()[2] != 1:
+        if len(t.shape) != 3 or t.shape[:2] != (batch, self.kv_heads) or t.shape[2] < 1 or t.stride()[2] != 1:
             raise _invalid(f"{name} must be f32 [{batch}, {self.kv_heads}, columns] with dense rows, "
                            f"got shape {tuple(t.shape)}")
         s = t.stride()
@@ -182,10 +166,10 @@ class PagedKV:
         kp, ks = self._rows(k, "k", n, self.kv_heads, None)
         vp, vs = self._rows(v, "v", n, self.kv_heads, _code(k))
         tp, ts, batch, cols = self._table(block_table, "block_table")
-        a = _Append(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), kp, vp, _code(k), ks, vs, n,
-                    None if sequences is None else self._ints(sequences, "sequences", n),
-                    self._ints(positions, "positions", n), tp, ts, cols, batch)
-        self._check(self._lib.gawee_kv_append(self._h, ctypes.byref(a), _stream_ptr(stream)))
+        a = _APPEND.pack(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), kp, vp, _code(k), ks, vs, n,
+                         0 if sequences is None else self._ints(sequences, "sequences", n),
+                         self._ints(positions, "positions", n), tp, ts, cols, batch)
+        self._check(self._lib.gawee_kv_append(self._h, a, _stream_ptr(stream)))
 
     def attend(self, k_pages, v_pages, q, block_table, lengths, out, scale: Optional[float] = None, k=None, v=None,
                mask=None, weights=None, weights_out=None, stream=None):
@@ -204,7 +188,7 @@ class PagedKV:
         tp, ts, rows, cols = self._table(block_table, "block_table")
         if rows != batch:
             raise _invalid(f"block_table has {rows} rows, q has {batch}")
-        kp = vp = mp = wp = wop = None
+        kp = vp = mp = wp = wop = 0
         ks = vs = ms = mc = ws = wb = wos = wob = wc = 0
         if k is not None:
             kp, ks = self._rows(k, "k", batch, self.kv_heads, code)
@@ -221,10 +205,11 @@ class PagedKV:
             wp, ws, wb, c = self._weights(weights, "weights", batch)
             if weights_out is not None and c != wc:
                 raise _invalid(f"weights has {c} columns, weights_out {wc}")
-        a = _Attend(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), qp, op, code, qs, os_, batch,
-                    self.head_dim ** -0.5 if scale is None else scale, tp, ts, cols,
-                    self._ints(lengths, "lengths", batch), kp, vp, ks, vs, mp, ms, mc, wp, ws, wb, wop, wos, wob, wc)
-        self._check(self._lib.gawee_kv_attend(self._h, ctypes.byref(a), _stream_ptr(stream)))
+        a = _ATTEND.pack(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), qp, op, code, qs, os_, batch,
+                         self.head_dim ** -0.5 if scale is None else scale, tp, ts, cols,
+                         self._ints(lengths, "lengths", batch), kp, vp, ks, vs, mp, ms, mc, wp, ws, wb, wop, wos, wob,
+                         wc)
+        self._check(self._lib.gawee_kv_attend(self._h, a, _stream_ptr(stream)))
         return out
 
     def evict(self, k_pages, v_pages, weights, block_table, lengths, budget: int, recent: int, kept, weights_out,
@@ -239,20 +224,20 @@ class PagedKV:
         wop, wos, wob, c = self._weights(weights_out, "weights_out", batch)
         if c != wc:
             raise _invalid(f"weights has {wc} columns, weights_out {c}")
-        if tuple(kept.shape) != (batch, self.kv_heads, budget) or not kept.is_contiguous():
+        if kept.shape != (batch, self.kv_heads, budget) or not kept.is_contiguous():
             raise _invalid(f"kept must be dense int32 {(batch, self.kv_heads, budget)}, got shape {tuple(kept.shape)}")
         if not 0 <= recent <= budget:
             raise _invalid(f"recent is {recent}, outside 0 .. {budget}")
-        top = None
-        tos = toc = 0
+        top = tos = toc = 0
         if to_table is not None:
             top, tos, rows, toc = self._table(to_table, "to_table")
             if rows != batch:
                 raise _invalid(f"to_table has {rows} rows, block_table {batch}")
-        a = _Evict(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), wp, ws, wb, wop, wos, wob, wc,
-                   batch, tp, ts, cols, top, tos, toc, self._ints(lengths, "lengths", batch),
-                   self._ints(lengths_out, "lengths_out", batch), budget, recent, self._on_device(kept, "kept", 4))
-        self._check(self._lib.gawee_kv_evict(self._h, ctypes.byref(a), _stream_ptr(stream)))
+        a = _EVICT.pack(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), wp, ws, wb, wop, wos, wob, wc,
+                        batch, tp, ts, cols, top, tos, toc, self._ints(lengths, "lengths", batch),
+                        self._ints(lengths_out, "lengths_out", batch), budget, recent,
+                        self._on_device(kept, "kept", 4))
+        self._check(self._lib.gawee_kv_evict(self._h, a, _stream_ptr(stream)))
 
     def synchronize(self, stream=None):
         """Wait for `stream` and raise what a call found wrong on the device since the last check."""

@@ -58,6 +58,7 @@ def load_library(path: str = LIB_PATH):
             "gawee_output_info": (c.c_int, [P, c.c_int, c.POINTER(c.c_int), c.POINTER(c.c_int), c.POINTER(c.c_int64)]),
             "gawee_set_arg": (c.c_int, [P, c.c_int, P, c.c_size_t, P]),
             "gawee_set_arg_device": (c.c_int, [P, c.c_int, P, c.c_size_t, P]),
+            "gawee_arg_device_ptr": (c.c_int, [P, c.c_int, c.POINTER(P)]),
             "gawee_forward": (c.c_int, [P, P]),
             "gawee_get_output": (c.c_int, [P, c.c_int, P, c.c_size_t, P]),
             "gawee_output_device_ptr": (c.c_int, [P, c.c_int, c.POINTER(P)]),
@@ -191,6 +192,12 @@ class Model:
 
     def set_arg_device(self, i: int, ptr: int, nbytes: int, stream=None):
         self._check(self._lib.gawee_set_arg_device(self._h, i, ptr, nbytes, _stream_ptr(stream)))
+
+    def arg_ptr(self, i: int) -> int:
+        """Device address of argument i, e.g. the pages of a paged_attention op."""
+        p = ctypes.c_void_p()
+        self._check(self._lib.gawee_arg_device_ptr(self._h, i, ctypes.byref(p)))
+        return p.value
 
     def set_args(self, arrays: Sequence[np.ndarray]):
         if len(arrays) != len(self.arg_specs):

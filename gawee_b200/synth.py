@@ -311,6 +311,10 @@ class GraphBuilder:
     def softmax(self, x, axis=-1):
         return self.op("softmax", [x], {"axis": f"{axis % len(x.shape)} : i64"}, x.dtype, x.shape)
 
+    def paged_attention(self, q, k, v, k_pages, v_pages, table, lengths, scale: float):
+        return self.op("paged_attention", [q, k, v, k_pages, v_pages, table, lengths],
+                       {"scale": f"{scale!r} : f64"}, q.dtype, q.shape)
+
     def gather(self, data, idx, axis=0):
         shape = data.shape[:axis] + idx.shape + data.shape[axis + 1:]
         return self.op("gather", [data, idx], {"axis": f"{axis} : i64"}, data.dtype, shape)
@@ -648,6 +652,55 @@ def llama_decode(batch: int = 1, past: int = 1, dim: int = 288, layers: int = 6,
     outs = [logits] + (presents if present else [])
     return SynthGraph(f"{name}_b{batch}_p{past}", g.finish(outs), g.args, [o.shape for o in outs], 5e-4,
                       batch, 1, flops[0])
+
+
+def llama_decode_paged(batch: int = 1, page_size: int = 16, max_pages: int = 16, num_pages: Optional[int] = None,
+                       length: int = 1, dim: int = 288, layers: int = 6, heads: int = 6,
+                       kv_heads: Optional[int] = None, ffn: int = 768, vocab: int = 32000, eps: float = 1e-5,
+                       theta: float = 10000.0, seed: int = 42, name: str = "llama15m_decode_paged") -> SynthGraph:
+    """llama_decode's step on a paged key/value cache: one graph, and one
+    captured CUDA graph, for every cache length.  Inputs: input_ids [B, 1],
+    position_ids [B, 1], block_table i32 [B, max_pages], lengths i32 [B] (rows
+    cached, the new token's among them), then per layer the key and value pages
+    [num_pages, kv_heads, page_size, head_dim], which stay in the context and take the
+    new rows in place.  Output: logits [B, 1, vocab].  Same weights as llama_decode."""
+    kv_heads = kv_heads or heads
+    hd = dim // heads
+    num_pages = num_pages or batch * max_pages
+    g = GraphBuilder(f"synthetic:{name}_b{batch}_{max_pages}x{page_size}", seed)
+    flops = [0]
+    ids_v = np.random.default_rng(seed + 1).integers(0, vocab, (batch, 1), dtype=np.int64)
+    ids = g.input("i64", (batch, 1), lambda: ids_v)
+    pid = g.input("i64", (batch, 1), lambda: np.full((batch, 1), length - 1, np.int64))
+    table = g.input("i32", (batch, max_pages),
+                    lambda: (np.arange(batch * max_pages, dtype=np.int32) % num_pages).reshape(batch, max_pages))
+    lens = g.input("i32", (batch,), lambda: np.full((batch,), length, np.int32))
+    shape = (num_pages, kv_heads, page_size, hd)
+    pages = [tuple(g.input("f32", shape, lambda: np.zeros(shape, np.float32)) for _ in range(2)) for _ in range(layers)]
+    emb = g.normal((vocab, dim), 0.02)
+    h = g.gather(emb, ids)                                                  # [B,1,dim]
+    inv = g.const((1.0 / (theta ** (np.arange(0, hd, 2, dtype=np.float64) / hd))).astype(np.float32).reshape(1, hd // 2), "f32")
+    freqs = g.mul(g.unsqueeze(g.cast(pid, 1, "f32"), [2]), inv)             # [B,1,hd/2]
+    embp = g.cat([freqs, freqs], 2)                                         # [B,1,hd]
+    cos = g.unsqueeze(g.cos(embp), [1])                                     # [B,1,1,hd]
+    sin = g.unsqueeze(g.sin(embp), [1])
+    for li in range(layers):
+        x = _rms_norm(g, h, eps)
+        q = g.transpose(g.reshape(_dense(g, x, dim, heads * hd, flops, False), (batch, 1, heads, hd)), [0, 2, 1, 3])
+        k = g.transpose(g.reshape(_dense(g, x, dim, kv_heads * hd, flops, False), (batch, 1, kv_heads, hd)), [0, 2, 1, 3])
+        v = g.reshape(_dense(g, x, dim, kv_heads * hd, flops, False), (batch, kv_heads, hd))
+        q = g.reshape(g.add(g.mul(q, cos), g.mul(_rotate_half(g, q), sin)), (batch, heads, hd))
+        k = g.reshape(g.add(g.mul(k, cos), g.mul(_rotate_half(g, k), sin)), (batch, kv_heads, hd))
+        o = g.reshape(g.paged_attention(q, k, v, *pages[li], table, lens, 1.0 / math.sqrt(hd)), (batch, 1, heads * hd))
+        h = g.add(h, _dense(g, o, heads * hd, dim, flops, False))
+        x = _rms_norm(g, h, eps)
+        gate = _dense(g, x, dim, ffn, flops, False)
+        up = _dense(g, x, dim, ffn, flops, False)
+        h = g.add(h, _dense(g, g.mul(g.mul(gate, g.sigmoid(gate)), up), ffn, dim, flops, False))
+    h = _rms_norm(g, h, eps)
+    flops[0] += 2 * batch * dim * vocab
+    logits = g.matmul(h, g.transpose(emb, [1, 0]))
+    return SynthGraph(f"{name}_b{batch}", g.finish([logits]), g.args, [logits.shape], 5e-4, batch, 1, flops[0])
 
 
 def llama15m_decode(batch: int = 1, past: int = 1, **kw) -> SynthGraph:

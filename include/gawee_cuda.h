@@ -88,6 +88,12 @@ gawee_status gawee_set_arg(gawee_ctx* ctx, int i, const void* host, size_t bytes
 /* Stage argument i from device memory on the context's device. */
 gawee_status gawee_set_arg_device(gawee_ctx* ctx, int i, const void* dev, size_t bytes, void* stream);
 
+/* Device pointer of argument i, in the context's memory until it is destroyed: for
+ * the pages of a gawee.paged_attention op, which the forward updates in place and
+ * the gawee_kv calls below can fill and evict from.  An argument that is a
+ * packed weight is written with gawee_set_arg instead. */
+gawee_status gawee_arg_device_ptr(gawee_ctx* ctx, int i, void** ptr);
+
 /* Enqueue one forward on `stream`.  Replaces the call of
  * _mlir_ciface_forward (back/gawee_aot.cpp:263-274).  Asynchronous. */
 gawee_status gawee_forward(gawee_ctx* ctx, void* stream);
@@ -224,6 +230,11 @@ gawee_status gawee_matmul_f32_noalloc(const float* a, const float* b, float* c, 
  * slot i % page_size of page table[b][i / page_size].  Columns behind a
  * sequence's last row are never read.  Lengths and tables are read on the
  * device when the call runs, so that one captured call serves every step.
+ *
+ * In a graph, gawee.paged_attention(q, k, v, k_pages, v_pages, block_table,
+ * lengths) <{scale}> is gawee_kv_attend with k and v: f32, the table and lengths i32,
+ * the pages two function arguments that nothing else uses; they live in the context and
+ * keep the stored rows from one forward to the next.
  *
  * A gawee_kv handle holds the shapes and the scratch memory, allocated once;
  * one handle serves any number of layers.

@@ -711,3 +711,91 @@ def test_prompts_steps_and_eviction_together(dtype, act):
                     assert torch.equal(c.get(pages, i, min(ln, budget)), c.rows[i][which])
             c.lens = lens.cpu().tolist()
             assert max(c.lens) <= budget
+
+
+# --- in a graph ------------------------------------------------------------------
+
+@pytest.mark.parametrize("graph_mode", [True, False], ids=["graph", "eager"])
+@pytest.mark.parametrize("kv_heads,page_size", [(2, 16), (4, 7)])
+def test_decode_graph_follows_the_concatenating_step_for_every_length(kv_heads, page_size, graph_mode):
+    """One context of llama_decode_paged against the oracle's run of llama_decode
+    (the same weights, the cache concatenated), one graph per length."""
+    import oracle
+    from gawee_b200 import synth
+    from gawee_b200.runtime import Model
+    from tests.helpers import compare
+    batch, layers, heads, dim, start = 2, 2, 4, 128, 3
+    kw = dict(batch=batch, dim=dim, layers=layers, heads=heads, kv_heads=kv_heads, ffn=128, vocab=300)
+    hd, cols = dim // heads, 4
+    g = synth.llama_decode_paged(page_size=page_size, max_pages=cols, num_pages=batch * cols + 1, **kw)
+    args = g.make_args()
+    rng = np.random.default_rng(50)
+    perm = rng.permutation(batch * cols + 1).astype(np.int32)[:batch * cols].reshape(batch, cols)
+    past = [rng.standard_normal((batch, kv_heads, start, hd), dtype=np.float32) for _ in range(2 * layers)]
+    args[2] = perm
+    for i, p in enumerate(past):  # rows 0 .. start - 1 of every layer
+        for b in range(batch):
+            for r in range(start):
+                args[4 + i][perm[b, r // page_size], :, r % page_size] = p[b, :, r]
+    m = Model(g.mlir, graph_mode=graph_mode)
+    try:
+        m.set_args(args)
+        for step in range(20):
+            n = start + step  # rows cached before this step
+            ids = rng.integers(0, 300, (batch, 1), dtype=np.int64)
+            pid = np.full((batch, 1), n, np.int64)
+            m.set_arg(0, ids)
+            m.set_arg(1, pid)
+            m.set_arg(3, np.full((batch,), n + 1, np.int32))
+            m.forward()
+            got = m.output(0)
+            m.synchronize()
+            ref = synth.llama_decode(past=n, **kw)
+            ra = ref.make_args()
+            weights = [a for a, s in zip(ra, ref.args) if s.kind == "weight"]
+            assert all(np.array_equal(a, b) for a, b in
+                       zip(weights, [a for a, s in zip(args, g.args) if s.kind == "weight"]))
+            want = oracle.run(ref.mlir, [ids, np.ones((batch, n + 1), np.int64), pid] + past + weights)
+            past = list(want[1:])
+            compare(got, want[0], atol=5e-4, rtol=1e-4, what=f"logits of step {step}")
+    finally:
+        m.close()
+
+
+def test_decode_graph_of_the_15m_shapes_runs_with_the_library_calls_on_its_pages():
+    """A prompt appended by gawee_kv_append into the context's own pages, then a step of the graph."""
+    from gawee_b200 import runtime, synth
+    from gawee_b200.paged_kv import _APPEND, PagedKV
+    from gawee_b200.runtime import Model
+    g = synth.llama_decode_paged(batch=1, layers=2, vocab=1000, page_size=16, max_pages=4)
+    args = g.make_args()
+    prompt = 37
+    rng = np.random.default_rng(51)
+    rows = [torch.from_numpy(rng.standard_normal((prompt, 6, 48), dtype=np.float32)).cuda() for _ in range(4)]
+    args[3][:] = prompt + 1
+    args[1][:] = prompt
+    plain = [a.copy() for a in args]
+    for i, r in enumerate(rows):
+        for j in range(prompt):
+            plain[4 + i][args[2][0, j // 16], :, j % 16] = r[j].cpu().numpy()
+    a, b = Model(g.mlir), Model(g.mlir)
+    try:
+        a.set_args(args)
+        kv = PagedKV("f32", 6, 6, 48, 16, 4, max_batch=1, max_pages=4)
+        table = torch.from_numpy(args[2]).cuda()
+        pos = torch.arange(prompt, dtype=torch.int32, device="cuda")
+        seq = torch.zeros(prompt, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        for layer in range(2):
+            packed = _APPEND.pack(a.arg_ptr(4 + 2 * layer), a.arg_ptr(5 + 2 * layer), rows[2 * layer].data_ptr(),
+                                  rows[2 * layer + 1].data_ptr(), 0, 288, 288, prompt, seq.data_ptr(), pos.data_ptr(),
+                                  table.data_ptr(), 4, 4, 1)
+            assert runtime.load_library().gawee_kv_append(kv._h, packed, None) == 0
+        kv.synchronize()
+        a.forward()
+        got = a.output(0)
+        want = b.run(plain)[0]
+        assert np.array_equal(got, want)
+    finally:
+        a.close()
+        b.close()

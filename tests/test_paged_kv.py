@@ -215,3 +215,72 @@ int main() {
     subprocess.run(["g++", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
                     os.path.join(build.CSRC, "kernels"), str(src), "-o", str(exe)], check=True)
     subprocess.run([str(exe)], check=True)
+
+
+def test_packed_arguments_have_the_layout_of_the_header(tmp_path):
+    from gawee_b200 import paged_kv
+    src = tmp_path / "s.cpp"
+    src.write_text("""
+#include <cstdio>
+#include "gawee_cuda.h"
+int main() {
+  printf("%zu %zu %zu %zu %zu %zu %zu\\n", sizeof(gawee_kv_desc), sizeof(gawee_kv_append_args), sizeof(gawee_kv_attend_args),
+         sizeof(gawee_kv_evict_args), offsetof(gawee_kv_attend_args, weights_cols), offsetof(gawee_kv_append_args, batch),
+         offsetof(gawee_kv_evict_args, kept));
+}
+""")
+    exe = tmp_path / "s"
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(build.ROOT, "include"), "-include", "cstddef", str(src), "-o",
+                    str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    structs = [paged_kv._DESC, paged_kv._APPEND, paged_kv._ATTEND, paged_kv._EVICT]
+    assert [(-(-s.size // 8)) * 8 for s in structs] == got[:4]
+    assert got[4:] == [paged_kv._ATTEND.size - 8, paged_kv._APPEND.size - 4, paged_kv._EVICT.size - 8]
+
+
+def _graph(**kw):
+    from gawee_b200 import synth
+    return synth.llama_decode_paged(batch=2, layers=2, heads=4, kv_heads=2, dim=128, ffn=128, vocab=64, **kw).mlir
+
+
+def test_decode_graph_plans_and_merges_its_projections():
+    plan = runtime.plan_text(_graph()).split()
+    assert plan.count("paged_attention") == 2 and plan.count("matmul3") == 2
+
+
+def _op_graph(use_pages_again=False, twice=False, computed_pages=False, **kw):
+    """One paged_attention op over inputs of the given shapes."""
+    from gawee_b200.synth import GraphBuilder
+    s = dict(q=(B, H, D), k=(B, KV, D), v=(B, KV, D), k_pages=(PAGES, KV, PAGE, D), v_pages=(PAGES, KV, PAGE, D),
+             table=(B, COLS), lengths=(B,), table_type="i32", lengths_type="i32", pages_type="f32")
+    s.update(kw)
+
+    def make(g):
+        def x(name, dtype="f32"):
+            return g.input(dtype, s[name], lambda: None)
+        q, k, v, kp, vp = x("q"), x("k"), x("v"), x("k_pages", s["pages_type"]), x("v_pages", s["pages_type"])
+        table, lengths = x("table", s["table_type"]), x("lengths", s["lengths_type"])
+        pages = g.relu(kp) if computed_pages else kp
+        out = [g.paged_attention(q, k, v, pages, kp if twice else vp, table, lengths, 0.5)]
+        return out + ([g.relu(vp)] if use_pages_again else [])
+    g = GraphBuilder("synthetic:test", 0)
+    return g.finish(make(g))
+
+
+def test_graph_op_plans():
+    assert "paged_attention" in runtime.plan_text(_op_graph())
+    assert "paged_attention" in runtime.plan_text(_op_graph(q=(B, 7 * KV, D)))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=(B, 5, D)), dict(q=(B + 1, H, D)), dict(q=(B, H, D + 8)), dict(q=(B * H, D)), dict(k=(B, KV + 1, D)),
+    dict(v=(B, KV, D, 1)), dict(k=(B, 2 * KV, D), v=(B, 2 * KV, D)), dict(table=(B + 1, COLS)), dict(table=(COLS,)),
+    dict(table_type="i64"), dict(lengths=(B + 1,)), dict(lengths=(B, 1)), dict(lengths_type="i64"),
+    dict(v_pages=(PAGES + 1, KV, PAGE, D)), dict(k_pages=(PAGES, PAGE, KV, D), v_pages=(PAGES, PAGE, KV, D)),
+    dict(q=(B, H, 12), k=(B, KV, 12), v=(B, KV, 12), k_pages=(PAGES, KV, PAGE, 12), v_pages=(PAGES, KV, PAGE, 12)),
+    dict(q=(B, H, 264), k=(B, KV, 264), v=(B, KV, 264), k_pages=(PAGES, KV, PAGE, 264), v_pages=(PAGES, KV, PAGE, 264)),
+    dict(pages_type="f64"), dict(use_pages_again=True), dict(twice=True), dict(computed_pages=True),
+])
+def test_graph_op_refuses(kw):
+    with pytest.raises(GaweeError, match="paged_attention"):
+        runtime.plan_text(_op_graph(**kw))
