@@ -35,9 +35,9 @@ Fn gather(const View& data, const View& idx, const View& out, int64_t pre, int64
 Fn gather_elements(const View& data, const View& idx, const View& out, int axis);
 Fn range(kern::RangeParams rp, const View& out);
 // One new token's attention over a paged key/value cache held in two arguments (kern::KvAttendParams):
-// q [B, H, D], k / v [B, Hkv, D], out dense; parts and arrived as kern::kv_parts_floats and kv_counters size them
+// q [B, H, D], k / v [B, Hkv, D], out dense; parts and info as kern::kv_parts_floats and kv_segments size them
 Fn paged_attention(const View& q, const View& k, const View& v, const View& k_pages, const View& v_pages,
-                   const View& table, const View& lengths, const View& out, const View& parts, const View& arrived,
+                   const View& table, const View& lengths, const View& out, const View& parts, const View& info,
                    float scale);
 Fn topk(const View& in, const View& vals, const View& idxs, const View& used, int64_t k);
 Fn pack(const PackSpec& ps, int64_t ldk, int hi, int lo);

@@ -23,7 +23,7 @@ struct gawee_kv {
   float* stats = nullptr;      // [max_batch][heads][2], with desc.weights
   float* scores = nullptr;     // [max_batch][heads][max_pages * page_size], with desc.weights
   float* parts = nullptr;      // attend's partial states
-  unsigned* arrived = nullptr; // attend's counters, 0 between calls
+  int2* info = nullptr;        // attend's segments and the blocks that share them
   int sms = 0;
   ~gawee_kv() {
     cudaFree(status);
@@ -31,7 +31,7 @@ struct gawee_kv {
     cudaFree(stats);
     cudaFree(scores);
     cudaFree(parts);
-    cudaFree(arrived);
+    cudaFree(info);
   }
 };
 
@@ -126,8 +126,8 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     if (!desc) return bad("null desc");
     const gawee_kv_desc& d = *desc;
     if (!is_act(d.dtype)) return bad("dtype must be f32, f16 or bf16");
-    if (d.kv_heads < 1 || d.kv_heads > 65535 || d.heads < d.kv_heads || d.heads > 65535 || d.heads % d.kv_heads)
-      return bad("heads must be a positive multiple of kv_heads");
+    if (d.kv_heads < 1 || d.heads < d.kv_heads || d.heads > 4096 || d.heads % d.kv_heads)
+      return bad("heads must be a positive multiple of kv_heads, up to 4096");
     if (d.head_dim < 8 || d.head_dim > 256 || d.head_dim % 8) return bad("head_dim must be a multiple of 8 up to 256");
     if (d.page_size < 1 || d.page_size > 65536) return bad("page_size must be 1 .. 65536");
     if (d.num_pages < 1 || d.num_pages > INT32_MAX) return bad("num_pages must be 1 .. 2^31 - 1");
@@ -140,7 +140,6 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     // lengths are int32; the kernels step past the last row by less than 2^20
     if (d.max_pages < 1 || (int64_t)d.max_pages * d.page_size > INT32_MAX - (1 << 20))
       return bad("max_pages * page_size must be 1 .. 2^31 - 2^20");
-    if ((int64_t)d.max_batch * d.heads > INT32_MAX / 2) return bad("max_batch * heads passes 2^30");
     auto kv = new gawee_kv();
     struct Drop {
       gawee_kv* kv;
@@ -170,9 +169,9 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     if (e == cudaSuccess)
       e = cudaMalloc((void**)&kv->parts,
                      sizeof(float) * gawee::kern::kv_parts_floats(kv->sms, d.heads / d.kv_heads, d.head_dim));
-    const size_t counters = sizeof(unsigned) * gawee::kern::kv_counters(kv->sms);
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->arrived, counters);
-    if (e == cudaSuccess) e = cudaMemset(kv->arrived, 0, counters);
+    if (e == cudaSuccess)
+      e = cudaMalloc((void**)&kv->info,
+                     sizeof(int2) * gawee::kern::kv_segments(d.max_batch, d.kv_heads, d.heads / d.kv_heads));
     if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
@@ -309,7 +308,7 @@ gawee_status gawee_kv_attend(gawee_kv* kv, const gawee_kv_attend_args* a, void* 
     p.scores = kv->scores;
     p.stats = kv->stats;
     p.parts = kv->parts;
-    p.arrived = kv->arrived;
+    p.info = kv->info;
     p.device = kv->device;
     p.sms = kv->sms;
     p.page_shift = gawee::kern::page_shift_of(kv->geom.page_size);

@@ -185,7 +185,6 @@ class Planner {
   std::unique_ptr<Plan> plan_;
   std::vector<bool> has_view_;
   std::set<int> page_bufs_;  // the pages arguments of paged_attention ops
-  int kv_counters_ = -1;     // their arrival counters' buffer
 
   // ---------------------------------------------------------------- attention clusters
   // matmul(Q, KT) -> div(A, c) [-> add(., mask)] -> softmax(-1) -> matmul(P, V),
@@ -1898,25 +1897,20 @@ class Planner {
     if (pages[1].shape != ps || ps[1] != KV || ps[3] != D || ps[2] < 1 || ps[2] > 65536)
       unsupported("paged_attention: the pages' shape does not match k and v");
     if (D < 8 || D > 256 || D % 8) unsupported("paged_attention: D must be a multiple of 8 up to 256");
-    if (B > 65535 || H > 65535 || ps[0] > INT32_MAX || table.shape[1] * ps[2] > INT32_MAX - (1 << 20))
+    if (B > 65535 || H > 4096 || ps[0] > INT32_MAX || table.shape[1] * ps[2] > INT32_MAX - (1 << 20))
       unsupported("paged_attention: batch, heads, pages or rows beyond the limits of gawee_kv_create");
     const Attr& sc = n.attr("scale");
     const double scale = sc.kind == Attr::INT ? (double)sc.i : sc.f;
     View out = alloc(DType::F32, val(n.outs[0]).type.shape);
     if (out.shape != q.shape) unsupported("paged_attention: the result has q's shape");
     View parts = alloc(DType::F32, {kern::kv_parts_floats(kern::kKvPlanSms, (int)(H / KV), (int)D)});
-    // counters that are 0 between calls; the calls of a forward follow one another, so one set serves them all
-    if (kv_counters_ < 0) {
-      kv_counters_ = new_buf(DType::I32, kern::kv_counters(kern::kKvPlanSms), BufKind::CONST);
-      plan_->bufs[kv_counters_].host_init.assign(4 * (size_t)kern::kv_counters(kern::kKvPlanSms), 0);
-    }
-    View arrived = dense_view(kv_counters_, DType::I32, {kern::kv_counters(kern::kKvPlanSms)});
+    View info = alloc(DType::I32, {2 * kern::kv_segments(B, (int)KV, (int)(H / KV))});
     Op op;
     op.kind = OpKind::PAGED_ATTN;
     op.name = "paged_attention";
-    op.reads = {q, k, v, pages[0], pages[1], table, lengths, arrived};
-    op.writes = {out, parts};
-    op.launch = launch::paged_attention(q, k, v, pages[0], pages[1], table, lengths, out, parts, arrived, (float)scale);
+    op.reads = {q, k, v, pages[0], pages[1], table, lengths};
+    op.writes = {out, parts, info};
+    op.launch = launch::paged_attention(q, k, v, pages[0], pages[1], table, lengths, out, parts, info, (float)scale);
     add_op(std::move(op));
     set_view(n.outs[0], out);
   }

@@ -1025,7 +1025,7 @@ Fn topk(const View& in, const View& vals, const View& idxs, const View& used, in
 }
 
 Fn paged_attention(const View& q, const View& k, const View& v, const View& k_pages, const View& v_pages,
-                   const View& table, const View& lengths, const View& out, const View& parts, const View& arrived,
+                   const View& table, const View& lengths, const View& out, const View& parts, const View& info,
                    float scale) {
   kern::KvAttendParams p{};
   const auto& ps = k_pages.shape;
@@ -1051,7 +1051,7 @@ Fn paged_attention(const View& q, const View& k, const View& v, const View& k_pa
     p.lengths = reinterpret_cast<const int32_t*>(rt.ptr(lengths));
     p.out = rt.ptr(out);
     p.parts = reinterpret_cast<float*>(rt.ptr(parts));
-    p.arrived = reinterpret_cast<unsigned*>(rt.ptr(arrived));
+    p.info = reinterpret_cast<int2*>(rt.ptr(info));
     p.status = rt.status();
     p.device = rt.device;
     if (!p.sms) GCHECK(cudaDeviceGetAttribute(&p.sms, cudaDevAttrMultiProcessorCount, rt.device));

@@ -19,8 +19,7 @@
 //   * Each warp keeps a running maximum, sum and weighted value sum (online
 //     softmax, fp32).  At the end of a segment the warps' states are joined in
 //     shared memory; a block that has only a part of the segment leaves its
-//     state in the workspace, and the block that arrives last joins the parts
-//     in their order, so the result does not depend on which block it is.
+//     state in the workspace, and kv_join_kernel (paged_kv.cu) joins the parts in their order.
 //
 // Rows that the mask takes out, rows behind the length and rows of bad pages
 // are not loaded: their stage rows are filled with zeros and their score is
@@ -43,16 +42,6 @@ constexpr int kMaxSmem = 220 * 1024;  // of a block, beside the kernel's static 
 constexpr int kMaxDevices = 64;
 
 // --- small pieces -------------------------------------------------------------
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// exp(s - m); a maximum of -inf (nothing attended yet) leaves exp(-inf) = 0, and NaN for a NaN score.
-__device__ __forceinline__ float exp_from(float s, float m) {
-  return exp2_fast((s - (m == -INFINITY ? 0.f : m)) * kLog2e);
-}
-
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // 16 bytes from global to shared memory; zeros where !valid (src is then not read).
@@ -87,13 +76,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-
-__device__ __forceinline__ void add_scaled(float4& to, const float4& x, float f) {
-  to.x += x.x * f;
-  to.y += x.y * f;
-  to.z += x.z * f;
-  to.w += x.w * f;
 }
 
 // --- the two ways to compute a tile ---------------------------------------------
@@ -575,21 +557,15 @@ inline int attend_smem(int row_bytes) {
   return kWarps * (P::kStages * (attend_stage_bytes<P>(row_bytes) + P::TK * 4) + P::kScratch * 4);
 }
 
-// Parts of a segment that one block joins at a time: with more of them, groups
-// of neighbours are joined first, each by the last of its blocks, then the
-// groups (one block that reads 148 parts takes longer than the attention).
-constexpr int kMostParts = 32;
-static_assert(kMostParts * kMostParts >= kKvMaxBlocksPerSm * 256, "two levels cover the grid");
-
 template <class P>
 __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(const __grid_constant__ KvAttendParams p) {
   using T = typename P::T;
   constexpr int TK = P::TK, TILE = kWarps * TK, NS = P::kStages, NH = P::NH;
   extern __shared__ __align__(128) char smem[];
   __shared__ long long s_warp[kWarps], s_base;
-  __shared__ int s_b0, s_last;
-  __shared__ float s_ml[kWarps][NH][2];           // the warps' maxima and sums
-  __shared__ float s_part[kMostParts][NH], s_top[NH][2];  // a join: the parts' factors, the result's maximum and sum
+  __shared__ int s_b0;
+  __shared__ float s_ml[kWarps][NH][2];  // the warps' maxima and sums
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may take its place early: it waits for this grid's end
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int D = P::kD ? P::kD : p.geom.head_dim, kv = p.geom.kv_heads, group = p.heads / kv, chunks = (group + NH - 1) / NH;
   const int per_tile = kv * chunks;  // segments of a sequence
@@ -849,33 +825,15 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     {
       // join the warps
       __syncthreads();
-      const long long seg_last = seg_begin + use.tiles - 1;
       const bool whole = seg_begin >= t0 && seg_end;
+      const int dv = D / 4;  // the results are taken four at a time
       // A part in the workspace: [NH][2], padded to 16 bytes, then [nh][D], counted
       // in units of 16 bytes.  A block has two places: 2 i + 1 for the segment that begins
       // in its run and goes on behind it, 2 i for the one that began before.
-      constexpr int kHead4 = (2 * NH + 3) / 4;
-      const int part4 = NH * D / 4 + kHead4;
-      float4* parts = reinterpret_cast<float4*>(p.parts);
-      const int dv = D / 4;  // the results are taken four at a time
-      auto finish = [&](int x, float mt, float lt, const float4& o) {
-        const int h = x / dv, d = x % dv * 4;
-        const int64_t at = use.b * p.out_stride + (int64_t)(h0 + h) * D + d;
-        const bool any = lt != 0.f;
-        store_act4(p.out, p.dt, at, any ? o.x / lt : 0.f, any ? o.y / lt : 0.f, any ? o.z / lt : 0.f, any ? o.w / lt : 0.f);
-        if (p.weights_out && d == 0) {
-          p.stats[((int64_t)use.b * p.heads + h0 + h) * 2] = mt;
-          p.stats[((int64_t)use.b * p.heads + h0 + h) * 2 + 1] = lt;
-        }
-      };
-      auto leave = [&](int place, int x, float mt, float lt, const float4& o) {
-        float4* q = parts + place * part4;
-        q[kHead4 + x] = o;
-        if (x % dv == 0) reinterpret_cast<float2*>(q)[x / dv] = make_float2(mt, lt);
-      };
-      const int own_place = 2 * blockIdx.x + (seg_begin >= t0 ? 1 : 0);
+      float4* part = reinterpret_cast<float4*>(p.parts) +
+                     (2 * blockIdx.x + (seg_begin >= t0 ? 1 : 0)) * kv_part_vecs(NH, D);
       for (int x = tid; x < nh * dv; x += kThreads) {
-        const int h = x / dv;
+        const int h = x / dv, d = x % dv * 4;
         float mt = -INFINITY, lt = 0.f;
         float4 ot = make_float4(0, 0, 0, 0);
 #pragma unroll
@@ -886,76 +844,19 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
           lt += s_ml[w][h][1] * c;
           add_scaled(ot, reinterpret_cast<const float4*>(smem + w * NS * stage_bytes + stage_at)[x], c);
         }
-        if (whole) finish(x, mt, lt, ot);
-        else leave(own_place, x, mt, lt, ot);
+        if (whole) store_result(p, use.b, h0 + h, d, mt, lt, ot);
+        else part[kv_part_head(NH) + x] = ot;
+        if (!whole && d == 0) reinterpret_cast<float2*>(part)[h] = make_float2(mt, lt);
       }
-      if (!whole) {
-        // The segment's blocks are c0 .. c1; the one that holds tile t is the
-        // largest i with floor(total * i / blocks) <= t.
-        const int c0 = (int)(((seg_begin + 1) * blocks - 1) / total);
-        const int n = (int)(((seg_last + 1) * blocks - 1) / total) - c0 + 1;
-        auto place_of = [&](int i) { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
-        int fan = kMostParts;  // parts of a group
-        if (n > kMostParts)
-          for (fan = 8; fan * fan < n;) fan *= 2;
-        const int me = blockIdx.x - c0;
-        for (int level = 0, step = 1; level < 2; ++level, step = fan) {
-          // this block's group: parts lo, lo + step, .. below hi; it is complete with its last arrival
-          const int lo = level == 0 ? me / fan * fan : 0, hi = level == 0 ? min(lo + fan, n) : n;
-          const int k = (hi - lo + step - 1) / step;
-          if (level == 1 && n <= fan) break;
-          __syncthreads();
-          if (tid == 0) {
-            // the fences are cumulative over the block's barriers; the counter wraps to
-            // 0 with the last arrival: ready for the next call
-            __threadfence();
-            s_last = k == 1 || atomicInc(p.arrived + 2 * place_of(lo) + level, k - 1) == (unsigned)(k - 1);
-            __threadfence();
-          }
-          __syncthreads();
-          if (!s_last) break;
-          if (k == 1) continue;
-          for (int h = warp; h < nh; h += kWarps) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + place_of(lo + min(lane, k - 1) * step) * part4) + h);
-            const float m = lane < k ? ml.x : -INFINITY, l = lane < k ? ml.y : 0.f;
-            float mt = m;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-            const float f = exp_from(m, mt);
-            float lt = l * f;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
-            s_part[lane][h] = f;  // 0 behind the last part
-            if (lane == 0) {
-              s_top[h][0] = mt;
-              s_top[h][1] = lt;
-            }
-          }
-          __syncthreads();
-          const bool done = level == 1 || n <= fan;
-          for (int x = tid; x < nh * dv; x += kThreads) {
-            const int h = x / dv;
-            float4 ot = make_float4(0, 0, 0, 0);
-            const float4* q = parts + kHead4 + x;
-            const int first_place = place_of(lo), stride = 2 * step * part4;
-            int at = 2 * (c0 + lo) * part4;
-            for (int i0 = 0; i0 < k; i0 += 8, at += 8 * stride) {  // eight loads on the way
-              float4 o[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (i0 + i < k) o[i] = __ldcg(q + (i0 + i == 0 ? first_place * part4 : at + i * stride));
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (i0 + i < k) add_scaled(ot, o[i], s_part[i0 + i][h]);
-            }
-            if (done) finish(x, s_top[h][0], s_top[h][1], ot);
-            else leave(first_place, x, s_top[h][0], s_top[h][1], ot);  // no other block reads that part any more
-          }
-        }
+      if (tid == 0 && seg_begin >= t0) {
+        // for the join: the segment's first block and the number of its blocks; the
+        // block that holds tile t is the largest i with floor(total * i / blocks) <= t
+        const int last = (int)(((seg_begin + use.tiles) * blocks - 1) / total);
+        p.info[((int64_t)use.b * kv + use.kvh) * chunks + use.chunk] = make_int2(blockIdx.x, last - (int)blockIdx.x + 1);
       }
       __syncthreads();  // the stages are free again
       if (padded) clear(ring + stage_at, stage_bytes);
-      seg_begin = seg_last + 1;
+      seg_begin += use.tiles;
     }
     if (j < count) advance(use);
   }
@@ -988,49 +889,51 @@ cudaError_t blocks_per_sm(int device, int smem, int* out) {
 }
 
 template <class P>
-cudaError_t attend_launch(const KvAttendParams& p, cudaStream_t s) {
+cudaError_t attend_launch(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
   const int D = p.geom.head_dim, smem = attend_smem<P>(P::row_bytes(D));
   int per_sm = 0;
   if (cudaError_t e = blocks_per_sm<P>(p.device, smem, &per_sm)) return e;
+  shape->heads = P::NH;
+  shape->split = p.max_len > kWarps * P::TK;
   kv_attend_kernel<P><<<p.sms * per_sm, kThreads, smem, s>>>(p);
   return cudaGetLastError();
 }
 
 // The kernel for these types, head dim and group.
 template <class T, int L, bool FULL>
-cudaError_t attend_lanes_group(const KvAttendParams& p, cudaStream_t s) {
+cudaError_t attend_lanes_group(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
   const int group = p.heads / p.geom.kv_heads;
-  if (group <= 1) return attend_launch<LaneTile<T, L, 1, FULL>>(p, s);
-  if (group <= 2) return attend_launch<LaneTile<T, L, 2, FULL>>(p, s);
+  if (group <= 1) return attend_launch<LaneTile<T, L, 1, FULL>>(p, shape, s);
+  if (group <= 2) return attend_launch<LaneTile<T, L, 2, FULL>>(p, shape, s);
   // a stage of four 16-bit rows has no room for the states of eight heads
   constexpr int kMost = L == 32 && sizeof(T) == 2 ? 4 : 8;
-  if (group <= 4) return attend_launch<LaneTile<T, L, 4, FULL>>(p, s);
-  return attend_launch<LaneTile<T, L, kMost, FULL>>(p, s);
+  if (group <= 4) return attend_launch<LaneTile<T, L, 4, FULL>>(p, shape, s);
+  return attend_launch<LaneTile<T, L, kMost, FULL>>(p, shape, s);
 }
 template <class T>
-cudaError_t attend_lanes(const KvAttendParams& p, cudaStream_t s) {
+cudaError_t attend_lanes(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
   const int D = p.geom.head_dim;
-  if (D <= 32) return attend_lanes_group<T, 4, false>(p, s);
-  if (D < 64) return attend_lanes_group<T, 8, false>(p, s);
-  if (D == 64) return attend_lanes_group<T, 8, true>(p, s);
-  if (D < 128) return attend_lanes_group<T, 16, false>(p, s);
-  if (D == 128) return attend_lanes_group<T, 16, true>(p, s);
-  return attend_lanes_group<T, 32, false>(p, s);
+  if (D <= 32) return attend_lanes_group<T, 4, false>(p, shape, s);
+  if (D < 64) return attend_lanes_group<T, 8, false>(p, shape, s);
+  if (D == 64) return attend_lanes_group<T, 8, true>(p, shape, s);
+  if (D < 128) return attend_lanes_group<T, 16, false>(p, shape, s);
+  if (D == 128) return attend_lanes_group<T, 16, true>(p, shape, s);
+  return attend_lanes_group<T, 32, false>(p, shape, s);
 }
 template <class T, int NH>
-cudaError_t attend_mma(const KvAttendParams& p, cudaStream_t s) {
+cudaError_t attend_mma(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
   const int D = p.geom.head_dim;
-  if (D < 64) return attend_launch<MmaTile<T, 64, NH, false>>(p, s);
-  if (D == 64) return attend_launch<MmaTile<T, 64, NH, true>>(p, s);
-  if (D < 128) return attend_launch<MmaTile<T, 128, NH, false>>(p, s);
-  if (D == 128) return attend_launch<MmaTile<T, 128, NH, true>>(p, s);
-  return attend_launch<MmaTile<T, 256, NH, false>>(p, s);
+  if (D < 64) return attend_launch<MmaTile<T, 64, NH, false>>(p, shape, s);
+  if (D == 64) return attend_launch<MmaTile<T, 64, NH, true>>(p, shape, s);
+  if (D < 128) return attend_launch<MmaTile<T, 128, NH, false>>(p, shape, s);
+  if (D == 128) return attend_launch<MmaTile<T, 128, NH, true>>(p, shape, s);
+  return attend_launch<MmaTile<T, 256, NH, false>>(p, shape, s);
 }
 template <class T>
-cudaError_t attend_16bit(const KvAttendParams& p, cudaStream_t s) {
+cudaError_t attend_16bit(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
   const int group = p.heads / p.geom.kv_heads;
-  if (p.dt == TypeCode<T>::value && group > 1) return group <= 8 ? attend_mma<T, 8>(p, s) : attend_mma<T, 16>(p, s);
-  return attend_lanes<T>(p, s);
+  if (p.dt == TypeCode<T>::value && group > 1) return group <= 8 ? attend_mma<T, 8>(p, shape, s) : attend_mma<T, 16>(p, shape, s);
+  return attend_lanes<T>(p, shape, s);
 }
 
 }  // namespace paged

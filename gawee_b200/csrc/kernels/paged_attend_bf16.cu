@@ -4,7 +4,9 @@
 namespace gawee {
 namespace kern {
 
-cudaError_t launch_kv_attend_bf16(const KvAttendParams& p, cudaStream_t s) { return paged::attend_16bit<__nv_bfloat16>(p, s); }
+cudaError_t launch_kv_attend_bf16(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
+  return paged::attend_16bit<__nv_bfloat16>(p, shape, s);
+}
 
 }  // namespace kern
 }  // namespace gawee

@@ -4,7 +4,9 @@
 namespace gawee {
 namespace kern {
 
-cudaError_t launch_kv_attend_f32(const KvAttendParams& p, cudaStream_t s) { return paged::attend_lanes<float>(p, s); }
+cudaError_t launch_kv_attend_f32(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
+  return paged::attend_lanes<float>(p, shape, s);
+}
 
 }  // namespace kern
 }  // namespace gawee

@@ -60,6 +60,32 @@ __device__ __forceinline__ void store_act4(void* p, int dt, int64_t i, float a, 
   else store4(static_cast<__nv_bfloat16*>(p) + i, a, b, c, d);
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// exp(s - m); a maximum of -inf (nothing attended yet) leaves exp(-inf) = 0, and NaN for a NaN score.
+__device__ __forceinline__ float exp_from(float s, float m) {
+  return exp2_fast((s - (m == -INFINITY ? 0.f : m)) * kLog2e);
+}
+__device__ __forceinline__ void add_scaled(float4& to, const float4& x, float f) {
+  to.x += x.x * f;
+  to.y += x.y * f;
+  to.z += x.z * f;
+  to.w += x.w * f;
+}
+
+// Elements d .. d + 3 of a head's result, from the sum of its weights `lt` (relative to their maximum `mt`).
+__device__ __forceinline__ void store_result(const KvAttendParams& p, int b, int head, int d, float mt, float lt,
+                                             const float4& o) {
+  const bool any = lt != 0.f;
+  store_act4(p.out, p.dt, b * p.out_stride + (int64_t)head * p.geom.head_dim + d, any ? o.x / lt : 0.f,
+             any ? o.y / lt : 0.f, any ? o.z / lt : 0.f, any ? o.w / lt : 0.f);
+  if (p.weights_out && d == 0)
+    reinterpret_cast<float2*>(p.stats)[(int64_t)b * p.heads + head] = make_float2(mt, lt);
+}
+
 }  // namespace paged
 }  // namespace kern
 }  // namespace gawee

@@ -1,5 +1,5 @@
-// Kernels of the paged key/value cache: append, the weights' pass of
-// attend (the attention itself is in paged_attend.cuh) and eviction by
+// Kernels of the paged key/value cache: append, the join and the
+// weights of attend (the attention itself is in paged_attend.cuh) and eviction by
 // accumulated attention weight.
 #include <cooperative_groups.h>
 
@@ -79,28 +79,109 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendParam
   }
 }
 
-// --- the weights of attend ------------------------------------------------------
-// weights_out = weights + the attention weights of this step, summed over the
-// query heads of the key/value head in their order.  Bound by the scores and
-// accumulators it reads and writes, which the attention left in L2.
-constexpr int kWeightThreads = 256;
+// --- the join of attend ------------------------------------------------------------
+//
+// A segment that several blocks of the attention shared is joined here, a
+// block per query head: the parts' maxima and sums give each part's factor, and groups of
+// threads add the scaled parts, in a fixed order.  Further blocks add the
+// weights of this step to their accumulators, over the query heads of a
+// key/value head in their order.  Both are short of work and bound by latency
+// (a block of the attention itself that joined 148 parts took 7 us more), so the
+// grid is launched while the attention runs and waits for its end.
+constexpr int kJoinThreads = 256;
 
-__global__ void __launch_bounds__(kWeightThreads) kv_weights_kernel(KvAttendParams p) {
-  extern __shared__ float2 s_head[];  // maximum and 1 / sum of each query head of the group
-  const int kvh = blockIdx.x % p.geom.kv_heads, b = blockIdx.x / p.geom.kv_heads;
-  const int group = p.heads / p.geom.kv_heads;
-  const int64_t len = p.lengths[b];
-  if (len > p.max_len || (int64_t)blockIdx.y * kWeightThreads >= len) return;
-  const float* stats = p.stats + ((int64_t)b * p.heads + kvh * group) * 2;
-  for (int g = threadIdx.x; g < group; g += kWeightThreads) s_head[g] = make_float2(stats[2 * g], 1.f / stats[2 * g + 1]);
+// A head's maximum and sum over its n parts, from the whole warp; `first` the segment's first block.
+__device__ __forceinline__ float2 join_stats(const KvAttendParams& p, int heads, int first, int n, int h) {
+  const int lane = threadIdx.x % 32, part = kv_part_vecs(heads, p.geom.head_dim);
+  const float4* parts = reinterpret_cast<const float4*>(p.parts);
+  float mt = -INFINITY, lt = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 128) {
+    float2 x[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = i0 + r * 32 + lane;
+      x[r] = i < n ? reinterpret_cast<const float2*>(parts + (i == 0 ? 2 * first + 1 : 2 * (first + i)) * part)[h]
+                   : make_float2(-INFINITY, 0.f);
+    }
+    float m = mt;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m = fmaxf(m, x[r].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    lt *= exp_from(mt, m);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lt += x[r].y * exp_from(x[r].x, m);
+    mt = m;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+  return make_float2(mt, lt);
+}
+
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ KvAttendParams p, int heads) {
+  extern __shared__ float4 s_join[];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the attention has ended and its results are visible
+  const int kv = p.geom.kv_heads, D = p.geom.head_dim, group = p.heads / kv, chunks = (group + heads - 1) / heads;
+  const int chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks, kvh = pair % kv, b = pair / kv;
+  const int tid = threadIdx.x, warp = tid / 32;
+  int len = p.lengths[b];
+  if (len < 0) return;
+  if (len > p.max_len) len = 0;
+  if ((int)blockIdx.y < heads) {
+    const int h = blockIdx.y, head = chunk * heads + h;
+    const int2 info = p.info[blockIdx.x];
+    if (head >= group || info.y <= 1) return;
+    const float2 top = join_stats(p, heads, info.x, info.y, h);  // every warp for itself
+    const int dv = D / 4, part = kv_part_vecs(heads, D);
+    int lanes = 2;  // threads of a group: one for each 16 bytes of the row
+    while (lanes < dv) lanes *= 2;
+    const int groups = kJoinThreads / lanes, g = tid / lanes, x = tid % lanes;
+    float4 sum = make_float4(0, 0, 0, 0);
+    if (x < dv) {
+      const float4* parts = reinterpret_cast<const float4*>(p.parts);
+      for (int i0 = g; i0 < info.y; i0 += 4 * groups) {
+        float4 o[4];
+        float f[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = i0 + r * groups;
+          const float4* q = parts + (i == 0 ? 2 * info.x + 1 : 2 * (info.x + i)) * part;
+          f[r] = i < info.y ? reinterpret_cast<const float2*>(q)[h].x : -INFINITY;
+          o[r] = i < info.y ? q[kv_part_head(heads) + h * dv + x] : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) add_scaled(sum, o[r], exp_from(f[r], top.x));
+      }
+      s_join[tid] = sum;
+    }
+    __syncthreads();
+    if (g == 0 && x < dv) {
+      for (int r = 1; r < groups; ++r) {
+        const float4 o = s_join[r * lanes + x];
+        add_scaled(sum, o, 1.f);
+      }
+      store_result(p, b, kvh * group + head, x * 4, top.x, top.y, sum);
+    }
+    return;
+  }
+  // the weights: blocks of the first chunk, each a stretch of the sequence
+  const int stretch = blockIdx.y - heads, stretches = gridDim.y - heads;
+  if (chunk != 0 || (int64_t)stretch * kJoinThreads >= len) return;
+  float2* s_head = reinterpret_cast<float2*>(s_join);  // maximum and 1 / sum of each query head of the group
+  for (int g = warp; g < group; g += kJoinThreads / 32) {
+    const int2 info = p.info[pair * chunks + g / heads];
+    const float2 top = info.y > 1 ? join_stats(p, heads, info.x, info.y, g % heads)
+                                  : reinterpret_cast<const float2*>(p.stats)[(int64_t)b * p.heads + kvh * group + g];
+    if (tid % 32 == 0) s_head[g] = make_float2(top.x, 1.f / top.y);
+  }
   __syncthreads();
-  for (int64_t i = (int64_t)blockIdx.y * kWeightThreads + threadIdx.x; i < len; i += (int64_t)gridDim.y * kWeightThreads) {
-    const float* s = p.scores + ((int64_t)blockIdx.x * p.max_len + i) * group;
+  for (int i = stretch * kJoinThreads + tid; i < len; i += stretches * kJoinThreads) {
+    const float* s = p.scores + ((int64_t)pair * p.max_len + i) * group;
     const float before = p.weights ? p.weights[b * p.w_batch + kvh * p.w_stride + i] : 0.f;
     float w = 0.f;
     for (int g = 0; g < group; ++g) {
-      const float2 h = s_head[g];
-      w += s[g] == -INFINITY ? 0.f : exp2f((s[g] - h.x) * kLog2e) * h.y;
+      const float2 t = s_head[g];
+      w += s[g] == -INFINITY ? 0.f : exp_from(s[g], t.x) * t.y;
     }
     p.weights_out[b * p.wo_batch + kvh * p.wo_stride + i] = before + w;
   }
@@ -389,19 +470,33 @@ cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t s) {
 
 cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s) {
   if (p.batch == 0) return cudaSuccess;
-  cudaError_t e = p.page_dt == DT_F32   ? launch_kv_attend_f32(p, s)
-                  : p.page_dt == DT_F16 ? launch_kv_attend_f16(p, s)
-                                        : launch_kv_attend_bf16(p, s);
-  if (e == cudaSuccess && p.weights_out) {
-    const int group = p.heads / p.geom.kv_heads, pairs = p.batch * p.geom.kv_heads;
+  KvAttendShape shape{};
+  cudaError_t e = p.page_dt == DT_F32   ? launch_kv_attend_f32(p, &shape, s)
+                  : p.page_dt == DT_F16 ? launch_kv_attend_f16(p, &shape, s)
+                                        : launch_kv_attend_bf16(p, &shape, s);
+  if (e != cudaSuccess || !(shape.split || p.weights_out)) return e;
+  const int group = p.heads / p.geom.kv_heads, chunks = (group + shape.heads - 1) / shape.heads;
+  const int pairs = p.batch * p.geom.kv_heads;
+  int stretches = 0;
+  size_t smem = sizeof(float4) * kJoinThreads;
+  if (p.weights_out) {
     // about eight blocks an SM over all pairs; a block beyond a sequence's end leaves at once
-    const int64_t most = (p.max_len + kWeightThreads - 1) / kWeightThreads;
+    const int64_t most = (p.max_len + kJoinThreads - 1) / kJoinThreads;
     const int64_t want = std::max<int64_t>(1, (8ll * p.sms + pairs - 1) / pairs);
-    kv_weights_kernel<<<dim3((unsigned)pairs, (unsigned)std::min<int64_t>(std::min(most, want), 65535)), kWeightThreads,
-                        sizeof(float2) * group, s>>>(p);
-    e = cudaGetLastError();
+    stretches = (int)std::min<int64_t>(std::min(most, want), 65535 - shape.heads);
+    smem = std::max(smem, sizeof(float2) * group);
   }
-  return e;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  cfg.gridDim = dim3((unsigned)(pairs * chunks), (unsigned)(shape.heads + stretches));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_join_kernel, p, shape.heads);
 }
 
 cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t s) {

@@ -15,12 +15,15 @@ namespace kern {
 // that an SM holds at most.  They size the workspace.
 constexpr int kKvHeadsMost = 16, kKvMaxBlocksPerSm = 4;
 
-// The attention's workspace on `sms` SMs: floats of the partial states, and
-// counters, 0 before the first call (every call leaves them 0).
+// The attention's workspace.  A part is the state of `heads` heads, in units of
+// 16 bytes: maxima and sums, then the weighted sums of values.
+GAWEE_HD int kv_part_head(int heads) { return (2 * heads + 3) / 4; }
+GAWEE_HD int kv_part_vecs(int heads, int head_dim) { return kv_part_head(heads) + heads * head_dim / 4; }
+// Floats of the parts on `sms` SMs, and segments (sequence, key/value head, chunk of heads).
 inline int64_t kv_parts_floats(int sms, int group, int head_dim) {
-  return (int64_t)2 * sms * kKvMaxBlocksPerSm * ((group > 8 ? kKvHeadsMost : 8) * (head_dim + 2) + 4);
+  return (int64_t)2 * sms * kKvMaxBlocksPerSm * 4 * kv_part_vecs(group > 8 ? kKvHeadsMost : 8, head_dim);
 }
-inline int64_t kv_counters(int sms) { return (int64_t)4 * sms * kKvMaxBlocksPerSm; }
+inline int64_t kv_segments(int64_t batch, int kv_heads, int group) { return batch * kv_heads * ((group + 3) / 4); }
 // SMs that a graph's workspace is planned for; a GPU with more uses this many.
 constexpr int kKvPlanSms = 160;
 
@@ -67,17 +70,21 @@ struct KvAttendParams {
   int64_t w_stride, w_batch, wo_stride, wo_batch;
   float* scores;         // [batch][kv_heads][max_len][heads / kv_heads], with weights_out
   float* stats;          // [batch][heads][2]: maximum and sum, with weights_out
-  float* parts;          // states of parts of segments: two a block, heads of a block * (D + 2) each
-  unsigned* arrived;     // two counters of arrivals a part; 0 between calls
+  float* parts;          // states of parts of segments: two a block
+  int2* info;            // of each segment: its first block, and the number of its blocks
   int device, sms;
   int page_shift;        // log2 of the page size, -1 where it is no power of two
   int* status;
 };
 cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s);
-// The same for pages of one type (paged_attend_*.cu), without the weights' pass.
-cudaError_t launch_kv_attend_f32(const KvAttendParams& p, cudaStream_t s);
-cudaError_t launch_kv_attend_f16(const KvAttendParams& p, cudaStream_t s);
-cudaError_t launch_kv_attend_bf16(const KvAttendParams& p, cudaStream_t s);
+// The same for pages of one type (paged_attend_*.cu), without the join.
+struct KvAttendShape {
+  int heads;   // of a part: the heads that a block computes together
+  bool split;  // a segment may have several tiles, and so several blocks
+};
+cudaError_t launch_kv_attend_f32(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s);
+cudaError_t launch_kv_attend_f16(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s);
+cudaError_t launch_kv_attend_bf16(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s);
 
 // Eviction by accumulated weight.
 struct KvEvictParams {
