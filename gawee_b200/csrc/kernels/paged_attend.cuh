@@ -10,7 +10,8 @@
 //     are cut into tiles, and all tiles of the batch, in order, are divided
 //     evenly over a fixed grid of resident blocks: a block takes a contiguous
 //     run of tiles, whatever the lengths are, and goes through several short
-//     segments or through a part of a long one.  The lengths are read on the
+//     segments or through a part of a long one.  A segment's begin and end cost
+//     about as much as a tile, and count as one.  The lengths are read on the
 //     device, so the balance needs nothing from the host.
 //   * A warp takes its own rows of each tile, through a ring of shared-memory
 //     stages of its own that cp.async fills: warps wait for no other until
@@ -545,6 +546,12 @@ template <int TILE>
 __device__ __forceinline__ int tiles_of(int len) {  // an empty sequence takes one, for its zeros
   return len < 0 ? 0 : len == 0 ? 1 : (len + TILE - 1) / TILE;
 }
+// Units of work of a segment: tile i is done by the block that has unit i + kStart.
+constexpr int kStart = 1;
+template <int TILE>
+__device__ __forceinline__ int units_of(int len) {
+  return len < 0 ? 0 : tiles_of<TILE>(len) + kStart;
+}
 
 // Shared memory in bytes: the warps' stages, their mask values and scratch.  At
 // the end of a segment a warp's state takes the place of the stage that it has just
@@ -571,11 +578,14 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   const int per_tile = kv * chunks;  // segments of a sequence
 
   // The block's run of tiles: prefix sums of the sequences' tiles, each thread a slice of the batch.
-  long long t0, t1, total, blocks;
+  long long u0, u1, total, blocks;  // its units
   {
     const int slice = (p.batch + kThreads - 1) / kThreads, b0 = min(tid * slice, p.batch), b1 = min(b0 + slice, p.batch);
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of<TILE>(length_of(p, b));
+    for (int b = b0; b < b1; ++b) {
+      mine += units_of<TILE>(length_of(p, b));
+      if (blockIdx.x == 0 && p.lengths[b] > p.max_len) set_status(p.status, ST_KV_LENGTH);  // length_of takes it as 0
+    }
     long long scan = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -590,16 +600,16 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
       sum += s_warp[w];
     }
     total = sum * per_tile;
-    blocks = min((long long)gridDim.x, total);  // every one of them has a tile
+    blocks = min((long long)gridDim.x, total);  // every one of them has a unit
     if (blockIdx.x >= blocks) return;
-    t0 = total * blockIdx.x / blocks;
-    t1 = total * (blockIdx.x + 1) / blocks;
+    u0 = total * blockIdx.x / blocks;
+    u1 = total * (blockIdx.x + 1) / blocks;
     before = (before + scan - mine) * per_tile;
-    if (t0 >= before && t0 < before + mine * per_tile) {  // this thread's slice holds the first tile
+    if (u0 >= before && u0 < before + mine * per_tile) {  // this thread's slice holds the first unit
       int b = b0;
       for (;; ++b) {
-        const long long n = (long long)tiles_of<TILE>(length_of(p, b)) * per_tile;
-        if (t0 < before + n) break;
+        const long long n = (long long)units_of<TILE>(length_of(p, b)) * per_tile;
+        if (u0 < before + n) break;
         before += n;
       }
       s_b0 = b;
@@ -631,14 +641,33 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   use.len = length_of(p, use.b);
   use.tiles = tiles_of<TILE>(use.len);
   {
-    const long long in = t0 - s_base;  // tiles into the sequence: (kvh, chunk, tile)
-    use.tile = (int)(in % use.tiles);
-    const int seg = (int)(in / use.tiles);
+    const long long in = u0 - s_base;  // units into the sequence: (kvh, chunk, unit)
+    const int units = use.tiles + kStart, seg = (int)(in / units), unit = (int)(in % units);
+    use.tile = max(unit - kStart, 0);
     use.chunk = seg % chunks;
     use.kvh = seg / chunks;
   }
+  long long seg_begin = 0;  // the segment's first unit
+  {
+    const int units = use.tiles + kStart;
+    seg_begin = s_base + ((long long)use.kvh * chunks + use.chunk) * units;
+  }
+  // tiles of the run: a walk over its segments
+  int count = 0;
+  {
+    Cursor c = use;
+    long long at = seg_begin;
+    for (;;) {
+      const long long end = at + kStart + c.tiles, upto = min(end, u1) - at - kStart;  // tiles of the segment before u1
+      if (upto > c.tile) count += (int)upto - c.tile;
+      at = end;
+      if (at >= u1) break;
+      c.tile = c.tiles - 1;
+      advance(c);
+    }
+  }
+  if (count == 0) return;  // a run of no more than the begin of a segment
   Cursor load = use;
-  const int count = (int)(t1 - t0);
 
   // the warp's part of shared memory
   const int rb = P::row_bytes(D), stage_bytes = attend_stage_bytes<P>(rb);
@@ -687,12 +716,13 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         }
       }
       if (lane < TK) adds[stage * TK + lane] = f_add;
-      const unsigned fresh_row = __ballot_sync(0xffffffffu, fresh);
-      const long long fresh_off = __shfl_sync(0xffffffffu, off, fresh_row ? __ffs(fresh_row) - 1 : 0);
+      unsigned fresh_row = 0;
+      long long fresh_off = 0;
+      if (p.k && first + TK >= c.len) {  // the tile of the last row
+        fresh_row = __ballot_sync(0xffffffffu, fresh);
+        fresh_off = __shfl_sync(0xffffffffu, off, fresh_row ? __ffs(fresh_row) - 1 : 0);
+      }
       if (f_add == -INFINITY || fresh) off = -1;  // nothing to load
-      // the new token's row is written below, unless the mask takes it out
-      const int new_row = fresh_row ? __ffs(fresh_row) - 1 : 0;
-      const bool put_new = fresh_row && __shfl_sync(0xffffffffu, f_add, new_row) != -INFINITY;
       if (__all_sync(0xffffffffu, off >= 0 || lane >= TK)) {  // whole rows: lane l takes vectors l, l + 32, ..
         const char* from = static_cast<const char*>(p.k_pages);
         const long long to_v = static_cast<const char*>(p.v_pages) - from;
@@ -728,6 +758,9 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         }
         return;
       }
+      // the new token's row is written below, unless the mask takes it out
+      const int new_row = fresh_row ? __ffs(fresh_row) - 1 : 0;
+      const bool put_new = fresh_row && __shfl_sync(0xffffffffu, f_add, new_row) != -INFINITY;
       int row = row_0, col = col_0;
       for (int v = 0; v < TK * vecs; v += 32) {
         const long long o = __shfl_sync(0xffffffffu, off, row & 31);
@@ -781,13 +814,12 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   }
 
   int stage = 0, load_stage = NS - 1;  // of the tile in use, and of the next tile to load
-  long long seg_begin = t0 - use.tile;  // the segment's first tile
   int j = 0;
 #pragma unroll 1
   while (j < count) {  // a segment, or the part of it that this block has
     const int h0 = use.kvh * group + use.chunk * NH, nh = min(NH, group - use.chunk * NH);
     const int mine = min(use.tiles - use.tile, count - j);
-    const bool seg_end = use.tile + mine == use.tiles;
+    const bool own_begin = use.tile == 0, seg_end = use.tile + mine == use.tiles;
     int stage_at = 0;
     {
       P state;
@@ -825,13 +857,13 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     {
       // join the warps
       __syncthreads();
-      const bool whole = seg_begin >= t0 && seg_end;
+      const bool begins = own_begin, whole = begins && seg_end;
       const int dv = D / 4;  // the results are taken four at a time
       // A part in the workspace: [NH][2], padded to 16 bytes, then [nh][D], counted
       // in units of 16 bytes.  A block has two places: 2 i + 1 for the segment that begins
       // in its run and goes on behind it, 2 i for the one that began before.
       float4* part = reinterpret_cast<float4*>(p.parts) +
-                     (2 * blockIdx.x + (seg_begin >= t0 ? 1 : 0)) * kv_part_vecs(NH, D);
+                     (2 * blockIdx.x + (begins ? 1 : 0)) * kv_part_vecs(NH, D);
       for (int x = tid; x < nh * dv; x += kThreads) {
         const int h = x / dv, d = x % dv * 4;
         float mt = -INFINITY, lt = 0.f;
@@ -848,22 +880,19 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         else part[kv_part_head(NH) + x] = ot;
         if (!whole && d == 0) reinterpret_cast<float2*>(part)[h] = make_float2(mt, lt);
       }
-      if (tid == 0 && seg_begin >= t0) {
+      if (tid == 0 && begins) {
         // for the join: the segment's first block and the number of its blocks; the
-        // block that holds tile t is the largest i with floor(total * i / blocks) <= t
-        const int last = (int)(((seg_begin + use.tiles) * blocks - 1) / total);
+        // block that holds unit u is the largest i with floor(total * i / blocks) <= u
+        const int last = (int)(((seg_begin + use.tiles + kStart) * blocks - 1) / total);
         p.info[((int64_t)use.b * kv + use.kvh) * chunks + use.chunk] = make_int2(blockIdx.x, last - (int)blockIdx.x + 1);
       }
       __syncthreads();  // the stages are free again
       if (padded) clear(ring + stage_at, stage_bytes);
-      seg_begin += use.tiles;
+      seg_begin += use.tiles + kStart;
     }
     if (j < count) advance(use);
   }
   copy_wait<0>();
-  if (blockIdx.x == 0)  // lengths that length_of took as 0
-    for (int b = tid; b < p.batch; b += kThreads)
-      if (p.lengths[b] > p.max_len) set_status(p.status, ST_KV_LENGTH);
 }
 
 // Blocks of this kernel that an SM holds, at most kMaxBlocksPerSm; asked once

@@ -120,40 +120,46 @@ __device__ __forceinline__ float2 join_stats(const KvAttendParams& p, int heads,
 
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ KvAttendParams p, int heads) {
   extern __shared__ float4 s_join[];
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the attention has ended and its results are visible
   const int kv = p.geom.kv_heads, D = p.geom.head_dim, group = p.heads / kv, chunks = (group + heads - 1) / heads;
   const int chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks, kvh = pair % kv, b = pair / kv;
   const int tid = threadIdx.x, warp = tid / 32;
-  int len = p.lengths[b];
+  int len = p.lengths[b];  // written before the attention began
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the attention has ended and its results are visible
   if (len < 0) return;
   if (len > p.max_len) len = 0;
   if ((int)blockIdx.y < heads) {
     const int h = blockIdx.y, head = chunk * heads + h;
     const int2 info = p.info[blockIdx.x];
     if (head >= group || info.y <= 1) return;
-    const float2 top = join_stats(p, heads, info.x, info.y, h);  // every warp for itself
     const int dv = D / 4, part = kv_part_vecs(heads, D);
     int lanes = 2;  // threads of a group: one for each 16 bytes of the row
     while (lanes < dv) lanes *= 2;
     const int groups = kJoinThreads / lanes, g = tid / lanes, x = tid % lanes;
     float4 sum = make_float4(0, 0, 0, 0);
-    if (x < dv) {
-      const float4* parts = reinterpret_cast<const float4*>(p.parts);
-      for (int i0 = g; i0 < info.y; i0 += 4 * groups) {
-        float4 o[4];
-        float f[4];
+    const float4* parts = reinterpret_cast<const float4*>(p.parts);
+    constexpr int kAtOnce = 8;
+    float4 o[kAtOnce];
+    float f[kAtOnce];
+    auto load = [&](int i0) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = i0 + r * groups;
-          const float4* q = parts + (i == 0 ? 2 * info.x + 1 : 2 * (info.x + i)) * part;
-          f[r] = i < info.y ? reinterpret_cast<const float2*>(q)[h].x : -INFINITY;
-          o[r] = i < info.y ? q[kv_part_head(heads) + h * dv + x] : make_float4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) add_scaled(sum, o[r], exp_from(f[r], top.x));
+      for (int r = 0; r < kAtOnce; ++r) {
+        const int i = i0 + r * groups;
+        const float4* q = parts + (i == 0 ? 2 * info.x + 1 : 2 * (info.x + i)) * part;
+        const bool in = i < info.y && x < dv;
+        f[r] = in ? reinterpret_cast<const float2*>(q)[h].x : -INFINITY;
+        o[r] = in ? q[kv_part_head(heads) + h * dv + x] : make_float4(0, 0, 0, 0);
       }
-      s_join[tid] = sum;
+    };
+    load(g);  // on the way while the statistics are formed
+    const float2 top = join_stats(p, heads, info.x, info.y, h);  // every warp for itself
+    for (int i0 = g;;) {
+#pragma unroll
+      for (int r = 0; r < kAtOnce; ++r) add_scaled(sum, o[r], exp_from(f[r], top.x));
+      i0 += kAtOnce * groups;
+      if (i0 >= info.y) break;
+      load(i0);
     }
+    s_join[tid] = sum;
     __syncthreads();
     if (g == 0 && x < dv) {
       for (int r = 1; r < groups; ++r) {
@@ -269,17 +275,25 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
     int* mine = hist[pass & 1];
     for (int i = tid; i < kBins; i += kSelectThreads) mine[i] = 0;
     __syncthreads();
-    for (int base = begin; base < old_end; base += kSelectThreads) {
-      const int i = base + tid;
-      const uint32_t k = i < old_end ? weight_key(w[i]) : 0u;
-      const bool in = i < old_end && (k & above) == prefix;
-      const int bin = in ? (int)((k >> shift) & ((1u << bits) - 1)) : -1;
-      int same;
-      __match_all_sync(0xffffffffu, bin, &same);
-      if (same) {  // many equal weights: one addition for the warp
-        if (bin >= 0 && tid % 32 == 0) atomicAdd(&mine[bin], 32);
-      } else if (bin >= 0) {
-        atomicAdd(&mine[bin], 1);
+    for (int base = begin; base < old_end; base += 8 * kSelectThreads) {
+      float x[8];  // eight loads on the way
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int i = base + r * kSelectThreads + tid;
+        x[r] = i < old_end ? w[i] : 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const uint32_t k = weight_key(x[r]);
+        const bool in = base + r * kSelectThreads + tid < old_end && (k & above) == prefix;
+        const int bin = in ? (int)((k >> shift) & ((1u << bits) - 1)) : -1;
+        int same;
+        __match_all_sync(0xffffffffu, bin, &same);
+        if (same) {  // many equal weights: one addition for the warp
+          if (bin >= 0 && tid % 32 == 0) atomicAdd(&mine[bin], 32);
+        } else if (bin >= 0) {
+          atomicAdd(&mine[bin], 1);
+        }
       }
     }
     cluster.sync();
@@ -306,21 +320,27 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
     // a block clears this histogram again only two passes on, behind the next cluster.sync
   }
   // keys above `prefix` and the recent rows stay for certain, and the first `need` of those equal to it
-  auto classify = [&](int i, int& sure, int& equal) {
-    sure = i < end && i >= cand;
-    equal = 0;
-    if (choose && i < old_end) {
-      const uint32_t k = weight_key(w[i]);
-      sure = k > prefix;
-      equal = k == prefix;
-    }
+  auto classify = [&](int i, float x, int& sure, int& equal) {
+    const uint32_t k = weight_key(x);
+    const bool old = choose && i < old_end;
+    sure = i < end && (i >= cand || (old && k > prefix));
+    equal = old && k == prefix;
   };
   int sure = 0, equal = 0;
-  for (int i = begin + tid; i < end; i += kSelectThreads) {
-    int a, e;
-    classify(i, a, e);
-    sure += a;
-    equal += e;
+  for (int base = begin; base < end; base += 8 * kSelectThreads) {
+    float x[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int i = base + r * kSelectThreads + tid;
+      x[r] = i < old_end ? w[i] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      int a, e;
+      classify(base + r * kSelectThreads + tid, x[r], a, e);
+      sure += a;
+      equal += e;
+    }
   }
   int all_sure, all_equal;
   block_scan(sure, warp_sums, all_sure);
@@ -339,9 +359,12 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
   constexpr int kEach = 4;  // consecutive positions of a thread
   for (int base = begin; base < end; base += kSelectThreads * kEach) {
     int a[kEach], e[kEach], packed = 0;
+    float y[kEach];
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) y[x] = base + tid * kEach + x < old_end ? w[base + tid * kEach + x] : 0.f;
 #pragma unroll
     for (int x = 0; x < kEach; ++x) {
-      classify(base + tid * kEach + x, a[x], e[x]);
+      classify(base + tid * kEach + x, y[x], a[x], e[x]);
       packed += a[x] | e[x] << 16;
     }
     int total;
