@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
 //   (kept for certain before it) + min(equal before it, equal ones that stay).
 // The weights are read five times, the first time from HBM, and the bound is the latency of the passes.
 constexpr int kSelectThreads = 1024;
-constexpr int kBins = 2048;
+constexpr int kBins = 2048, kMostBlocks = 8;  // of a cluster
 
 // Weights in ascending order of their values as unsigned integers; both zeros
 // are equal and NaN is below every number.
@@ -239,12 +239,14 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
 static_assert(kSelectThreads == 32 * 32, "block_scan takes one warp's lanes for the warps");
 
 __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
-  __shared__ int hist[2][kBins];
+  __shared__ __align__(16) int hist[2][kBins];
   __shared__ int warp_sums[32];
-  __shared__ int s_bin, s_need, s_sure, s_equal;
+  __shared__ int s_bin, s_need;
+  __shared__ int2 s_counts;
   const int pair = blockIdx.x / blocks;
   const int kvh = pair % p.geom.kv_heads, b = pair / p.geom.kv_heads;
   const int tid = threadIdx.x;
@@ -285,26 +287,22 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const uint32_t k = weight_key(x[r]);
-        const bool in = base + r * kSelectThreads + tid < old_end && (k & above) == prefix;
-        const int bin = in ? (int)((k >> shift) & ((1u << bits) - 1)) : -1;
-        int same;
-        __match_all_sync(0xffffffffu, bin, &same);
-        if (same) {  // many equal weights: one addition for the warp
-          if (bin >= 0 && tid % 32 == 0) atomicAdd(&mine[bin], 32);
-        } else if (bin >= 0) {
-          atomicAdd(&mine[bin], 1);
-        }
+        if (base + r * kSelectThreads + tid < old_end && (k & above) == prefix)
+          atomicAdd(&mine[(k >> shift) & ((1u << bits) - 1)], 1);
       }
     }
-    cluster.sync();
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
     // this thread's two bins, from the highest down
     const int hi = kBins - 1 - 2 * tid, lo = hi - 1;
     int h1 = 0, h0 = 0;
-    for (int r = 0; r < blocks; ++r) {
-      const int* theirs = cluster.map_shared_rank(mine, r);
-      h1 += theirs[hi];
-      h0 += theirs[lo];
-    }
+#pragma unroll
+    for (int r = 0; r < kMostBlocks; ++r)
+      if (r < blocks) {
+        const int2 x = *reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, r) + lo);
+        h1 += x.y;
+        h0 += x.x;
+      }
     int total;
     const int before = block_scan(h1 + h0, warp_sums, total);
     if (before < need && before + h1 >= need) {
@@ -326,36 +324,38 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
     sure = i < end && (i >= cand || (old && k > prefix));
     equal = old && k == prefix;
   };
-  int sure = 0, equal = 0;
-  for (int base = begin; base < end; base += 8 * kSelectThreads) {
-    float x[8];
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const int i = base + r * kSelectThreads + tid;
-      x[r] = i < old_end ? w[i] : 0.f;
-    }
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      int a, e;
-      classify(base + r * kSelectThreads + tid, x[r], a, e);
-      sure += a;
-      equal += e;
-    }
-  }
-  int all_sure, all_equal;
-  block_scan(sure, warp_sums, all_sure);
-  block_scan(equal, warp_sums, all_equal);
-  if (tid == 0) {
-    s_sure = all_sure;
-    s_equal = all_equal;
-  }
-  cluster.sync();
   int sure_before = 0, equal_before = 0;
-  for (int r = 0; r < rank; ++r) {
-    sure_before += *cluster.map_shared_rank(&s_sure, r);
-    equal_before += *cluster.map_shared_rank(&s_equal, r);
+  if (blocks > 1) {  // how many of each lie in the blocks before
+    int sure = 0, equal = 0;
+    for (int base = begin; base < end; base += 8 * kSelectThreads) {
+      float x[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int i = base + r * kSelectThreads + tid;
+        x[r] = i < old_end ? w[i] : 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        int a, e;
+        classify(base + r * kSelectThreads + tid, x[r], a, e);
+        sure += a;
+        equal += e;
+      }
+    }
+    int all_sure, all_equal;
+    block_scan(sure, warp_sums, all_sure);
+    block_scan(equal, warp_sums, all_equal);
+    if (tid == 0) s_counts = make_int2(all_sure, all_equal);
+    cluster.sync();
+#pragma unroll
+    for (int r = 0; r < kMostBlocks; ++r)
+      if (r < rank) {
+        const int2 x = *cluster.map_shared_rank(&s_counts, r);
+        sure_before += x.x;
+        equal_before += x.y;
+      }
+    cluster.sync();  // no block leaves while its shared memory is read
   }
-  cluster.sync();  // no block leaves while its shared memory is read
   constexpr int kEach = 4;  // consecutive positions of a thread
   for (int base = begin; base < end; base += kSelectThreads * kEach) {
     int a[kEach], e[kEach], packed = 0;
@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(KvEvictParams p, 
   const int kvh = blockIdx.x % p.geom.kv_heads, b = blockIdx.x / p.geom.kv_heads;
   const int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
   const int tid = threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the selection has ended
   if ((int)blockIdx.y == row_blocks) {  // the weights
     const int len = p.plan[2 * b], left = min(len, p.budget);
     if (kvh == 0 && tid == 0) p.lengths_out[b] = p.plan[2 * b + 1];
@@ -527,7 +528,7 @@ cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t s) {
   const int pairs = p.batch * p.geom.kv_heads;
   // Blocks of a pair's cluster: as many as the GPU holds at once, of 2048 positions at least.
   int cluster = 1;
-  while (cluster < 8 && (int64_t)pairs * cluster * 2 <= 2 * p.sms && p.max_len / (cluster * 2) >= 2 * kSelectThreads)
+  while (cluster < kMostBlocks && (int64_t)pairs * cluster * 2 <= 2 * p.sms && p.max_len / (cluster * 2) >= 2 * kSelectThreads)
     cluster *= 2;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
@@ -541,19 +542,25 @@ cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t s) {
   cfg.numAttrs = 1;
   if (cudaError_t e = cudaLaunchKernelEx(&cfg, kv_select_kernel, p)) return e;
 
+  // the move takes its place while the selection runs, and waits for its end
+  cfg.blockDim = dim3(kMoveThreads);
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+
   const int es = elem_bytes(p.page_dt), row_vecs = p.geom.head_dim * es / 16;
   if (p.to_table) {
     const int step = kMoveThreads / row_vecs * kMoveRows;
     const int64_t want = std::max<int64_t>(1, (16ll * p.sms + pairs - 1) / pairs);
     const int blocks = (int)std::min<int64_t>((p.budget + step - 1) / step, std::min<int64_t>(want, 65534));
-    kv_move_kernel<false><<<dim3((unsigned)pairs, (unsigned)blocks + 1), kMoveThreads, 0, s>>>(p, row_vecs, es, blocks);
+    cfg.gridDim = dim3((unsigned)pairs, (unsigned)blocks + 1);
+    return cudaLaunchKernelEx(&cfg, kv_move_kernel<false>, p, row_vecs, es, blocks);
   } else {
     int vecs = row_vecs;  // of a slice: halved while the slices leave SMs idle
     while (vecs % 2 == 0 && (int64_t)pairs * 2 * (row_vecs / vecs) < 8ll * p.sms) vecs /= 2;
     const int slices = row_vecs / vecs;
-    kv_move_kernel<true><<<dim3((unsigned)pairs, (unsigned)(2 * slices + 1)), kMoveThreads, 0, s>>>(p, vecs, es, 2 * slices);
+    cfg.gridDim = dim3((unsigned)pairs, (unsigned)(2 * slices + 1));
+    return cudaLaunchKernelEx(&cfg, kv_move_kernel<true>, p, vecs, es, 2 * slices);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace kern
