@@ -202,7 +202,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
 // weights stay from the lowest position on, so a kept row's new place is
 //   (kept for certain before it) + min(equal before it, equal ones that stay).
 // The weights are read five times, the first time from HBM, and the bound is the latency of the passes.
-constexpr int kSelectThreads = 1024;
+// A block that works alone ranks the last candidates directly as soon as no more
+// of them are left than it has threads: mostly after the first 11 bits.
 constexpr int kBins = 2048, kMostBlocks = 8;  // of a cluster
 
 // Weights in ascending order of their values as unsigned integers; both zeros
@@ -214,6 +215,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // Sums of x over the block's threads before this one, and over all; every thread calls it.
+template <int THREADS>
 __device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int scan = x;
@@ -225,7 +227,7 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
   __syncthreads();  // the last call's sums have been read
   if (lane == 31) warp_sums[warp] = scan;
   __syncthreads();
-  const int mine = warp_sums[lane];  // as many warps as lanes
+  const int mine = lane < THREADS / 32 ? warp_sums[lane] : 0;
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -236,16 +238,18 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
   const int before = __shfl_sync(0xffffffffu, upto - mine, warp);
   return before + scan - x;
 }
-static_assert(kSelectThreads == 32 * 32, "block_scan takes one warp's lanes for the warps");
 
-__global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams p) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_select_kernel(KvEvictParams p) {
   asm volatile("griddepcontrol.launch_dependents;");
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   __shared__ __align__(16) int hist[2][kBins];
   __shared__ int warp_sums[32];
-  __shared__ int s_bin, s_need;
+  __shared__ int s_bin, s_need, s_left;
+  __shared__ uint32_t s_key[THREADS];
+  __shared__ int s_at[THREADS];
   __shared__ int2 s_counts;
   const int pair = blockIdx.x / blocks;
   const int kvh = pair % p.geom.kv_heads, b = pair / p.geom.kv_heads;
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
     p.plan[2 * b + 1] = len > p.budget ? p.budget : p.lengths[b];
   }
   if (len <= p.budget) {  // the whole cluster
-    for (int j = rank * kSelectThreads + tid; j < p.budget; j += blocks * kSelectThreads) kept[j] = j < len ? j : -1;
+    for (int j = rank * THREADS + tid; j < p.budget; j += blocks * THREADS) kept[j] = j < len ? j : -1;
     return;
   }
   const float* w = p.weights + b * p.w_batch + kvh * p.w_stride;
@@ -275,47 +279,104 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     const uint32_t above = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
     int* mine = hist[pass & 1];
-    for (int i = tid; i < kBins; i += kSelectThreads) mine[i] = 0;
+    for (int i = tid; i < kBins; i += THREADS) mine[i] = 0;
     __syncthreads();
-    for (int base = begin; base < old_end; base += 8 * kSelectThreads) {
+    for (int base = begin; base < old_end; base += 8 * THREADS) {
       float x[8];  // eight loads on the way
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        const int i = base + r * kSelectThreads + tid;
+        const int i = base + r * THREADS + tid;
         x[r] = i < old_end ? w[i] : 0.f;
       }
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const uint32_t k = weight_key(x[r]);
-        if (base + r * kSelectThreads + tid < old_end && (k & above) == prefix)
+        if (base + r * THREADS + tid < old_end && (k & above) == prefix)
           atomicAdd(&mine[(k >> shift) & ((1u << bits) - 1)], 1);
       }
     }
     if (blocks > 1) cluster.sync();
     else __syncthreads();
-    // this thread's two bins, from the highest down
-    const int hi = kBins - 1 - 2 * tid, lo = hi - 1;
-    int h1 = 0, h0 = 0;
+    // this thread's bins, from the highest down
+    constexpr int kEach = kBins / THREADS;
+    const int lo = kBins - kEach * (tid + 1);
+    int h[kEach] = {}, sum = 0;
+    if (blocks == 1) {
 #pragma unroll
-    for (int r = 0; r < kMostBlocks; ++r)
-      if (r < blocks) {
-        const int2 x = *reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, r) + lo);
-        h1 += x.y;
-        h0 += x.x;
-      }
+      for (int x = 0; x < kEach; ++x) h[x] = mine[lo + x];
+    } else {
+#pragma unroll
+      for (int r = 0; r < kMostBlocks; ++r)
+        if (r < blocks) {
+          const int2* theirs = reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, r) + lo);
+#pragma unroll
+          for (int x = 0; x < kEach; x += 2) {
+            const int2 y = theirs[x / 2];
+            h[x] += y.x;
+            h[x + 1] += y.y;
+          }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) sum += h[x];
     int total;
-    const int before = block_scan(h1 + h0, warp_sums, total);
-    if (before < need && before + h1 >= need) {
-      s_bin = hi;
-      s_need = need - before;
-    } else if (before + h1 < need && before + h1 + h0 >= need) {
-      s_bin = lo;
-      s_need = need - before - h1;
+    int before = block_scan<THREADS>(sum, warp_sums, total);
+#pragma unroll
+    for (int x = kEach - 1; x >= 0; --x) {
+      if (before < need && before + h[x] >= need) {
+        s_bin = lo + x;
+        s_need = need - before;
+        s_left = h[x];
+      }
+      before += h[x];
     }
     __syncthreads();
     prefix |= (uint32_t)s_bin << shift;
     need = s_need;
     // a block clears this histogram again only two passes on, behind the next cluster.sync
+    if (blocks == 1 && shift && s_left <= THREADS) {
+      const int left = s_left;
+      __syncthreads();
+      if (tid == 0) s_left = 0;
+      __syncthreads();
+      const uint32_t upto = 0xffffffffu << shift;
+      for (int base = begin; base < old_end; base += 8 * THREADS) {
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int i = base + r * THREADS + tid;
+          x[r] = i < old_end ? w[i] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int i = base + r * THREADS + tid;
+          const uint32_t k = weight_key(x[r]);
+          if (i < old_end && (k & upto) == prefix) {
+            const int at = atomicAdd(&s_left, 1);
+            s_key[at] = k;
+            s_at[at] = i;
+          }
+        }
+      }
+      __syncthreads();
+      if (tid < left) {
+        const uint32_t k = s_key[tid];
+        const int i = s_at[tid];
+        int greater = 0, first = 0;
+        for (int x = 0; x < left; ++x) {
+          greater += s_key[x] > k;
+          first += s_key[x] == k && s_at[x] < i;
+        }
+        if (greater + first == need - 1) {  // the last one that stays
+          s_bin = (int)k;
+          s_need = need - greater;
+        }
+      }
+      __syncthreads();
+      prefix = (uint32_t)s_bin;
+      need = s_need;
+      break;
+    }
   }
   // keys above `prefix` and the recent rows stay for certain, and the first `need` of those equal to it
   auto classify = [&](int i, float x, int& sure, int& equal) {
@@ -327,24 +388,24 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
   int sure_before = 0, equal_before = 0;
   if (blocks > 1) {  // how many of each lie in the blocks before
     int sure = 0, equal = 0;
-    for (int base = begin; base < end; base += 8 * kSelectThreads) {
+    for (int base = begin; base < end; base += 8 * THREADS) {
       float x[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        const int i = base + r * kSelectThreads + tid;
+        const int i = base + r * THREADS + tid;
         x[r] = i < old_end ? w[i] : 0.f;
       }
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         int a, e;
-        classify(base + r * kSelectThreads + tid, x[r], a, e);
+        classify(base + r * THREADS + tid, x[r], a, e);
         sure += a;
         equal += e;
       }
     }
     int all_sure, all_equal;
-    block_scan(sure, warp_sums, all_sure);
-    block_scan(equal, warp_sums, all_equal);
+    block_scan<THREADS>(sure, warp_sums, all_sure);
+    block_scan<THREADS>(equal, warp_sums, all_equal);
     if (tid == 0) s_counts = make_int2(all_sure, all_equal);
     cluster.sync();
 #pragma unroll
@@ -357,7 +418,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
     cluster.sync();  // no block leaves while its shared memory is read
   }
   constexpr int kEach = 4;  // consecutive positions of a thread
-  for (int base = begin; base < end; base += kSelectThreads * kEach) {
+  for (int base = begin; base < end; base += THREADS * kEach) {
     int a[kEach], e[kEach], packed = 0;
     float y[kEach];
 #pragma unroll
@@ -368,7 +429,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(KvEvictParams
       packed += a[x] | e[x] << 16;
     }
     int total;
-    const int before = block_scan(packed, warp_sums, total);
+    const int before = block_scan<THREADS>(packed, warp_sums, total);
     int s = sure_before + (before & 0xffff), q = equal_before + (before >> 16);
 #pragma unroll
     for (int x = 0; x < kEach; ++x) {
@@ -397,11 +458,18 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(KvEvictParams p, 
   const int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
   const int tid = threadIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the selection has ended
+  const int len = p.plan[2 * b], left = max(min(len, p.budget), 0);
+  float* wo = p.weights_out + b * p.wo_batch + kvh * p.wo_stride;
+  // zeros from the new length to the old one: by all blocks, or, where the
+  // weights themselves are overwritten, by the block that has read them
+  const bool alone = p.weights == p.weights_out;
+  const int fill_blocks = alone ? 1 : row_blocks + 1, fill_block = alone ? 0 : (int)blockIdx.y;
+  auto fill = [&] {
+    for (int j = left + fill_block * kMoveThreads + tid; j < len; j += fill_blocks * kMoveThreads) wo[j] = 0.f;
+  };
   if ((int)blockIdx.y == row_blocks) {  // the weights
-    const int len = p.plan[2 * b], left = min(len, p.budget);
     if (kvh == 0 && tid == 0) p.lengths_out[b] = p.plan[2 * b + 1];
     const float* w = p.weights + b * p.w_batch + kvh * p.w_stride;
-    float* wo = p.weights_out + b * p.wo_batch + kvh * p.wo_stride;
     constexpr int kEach = 8;
     for (int j0 = 0; j0 < left; j0 += kMoveThreads * kEach) {
       float x[kEach];
@@ -418,9 +486,10 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(KvEvictParams p, 
       }
     }
     __syncthreads();
-    for (int j = max(left, 0) + tid; j < len; j += kMoveThreads) wo[j] = 0.f;
+    fill();
     return;
   }
+  if (!alone) fill();
   const int32_t* from = p.table + b * p.table_stride;
   const int32_t* to = IN_PLACE ? from : p.to_table + b * p.to_stride;
   const int64_t to_cols = IN_PLACE ? p.table_cols : p.to_cols;
@@ -526,21 +595,26 @@ cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s) {
 cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t s) {
   if (p.batch == 0) return cudaSuccess;
   const int pairs = p.batch * p.geom.kv_heads;
-  // Blocks of a pair's cluster: as many as the GPU holds at once, of 2048 positions at least.
+  // Threads of a block: 1024, or 256 where a thread then has 16 positions at
+  // most; eight such blocks on an SM hide each other's waits (450 pairs of 400
+  // rows: 11 us; with 1024 threads 31).  Blocks of a pair's cluster: doubled while each keeps 2048
+  // positions and the clusters of 1024 threads find room at once, at 96 blocks
+  // (8 pairs of 65,537 rows: 70 us alone, 39 with 4, 30 with 8; 20 pairs of
+  // 25,551: 44 us alone, 23 with 4, but 49 with 8, in two waves).
+  const bool small = p.max_len <= 4096;
   int cluster = 1;
-  while (cluster < kMostBlocks && (int64_t)pairs * cluster * 2 <= 2 * p.sms && p.max_len / (cluster * 2) >= 2 * kSelectThreads)
-    cluster *= 2;
+  while (!small && cluster < kMostBlocks && pairs * cluster * 2 <= 96 && p.max_len / (cluster * 2) >= 2048) cluster *= 2;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
   cfg.gridDim = dim3((unsigned)(pairs * cluster));
-  cfg.blockDim = dim3(kSelectThreads);
+  cfg.blockDim = dim3(small ? 256 : 1024);
   cfg.stream = s;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = (unsigned)cluster;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kv_select_kernel, p)) return e;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, small ? kv_select_kernel<256> : kv_select_kernel<1024>, p)) return e;
 
   // the move takes its place while the selection runs, and waits for its end
   cfg.blockDim = dim3(kMoveThreads);
