@@ -73,6 +73,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -81,196 +86,198 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 
 // --- the two ways to compute a tile ---------------------------------------------
 //
-// Lanes: any types.  L lanes hold a key's row, eight elements each (D <= 8 L),
-// and 32 / L keys are taken at a time.  All products in fp32, two to an
-// instruction.  The partial products of four keys a lane and NH heads are
-// summed over the L lanes by exchanging halves: after it each lane holds
-// complete scores of its own instead of all lanes holding all of them.
-// With FULL, D is 8 L: known to the compiler, no lane idle.
+// Lanes: any types, all products in fp32, two to an instruction.  A warp's tile
+// has TK = 128 / L keys of D <= 8 L elements: 8 KB of K and V in fp32, 4 KB in 16 bits.
+//   scores: W = L / 4 lanes share a key and take every W-th 16-byte chunk of its
+//     row; the query heads come from shared memory, the same address for all
+//     keys, so that a score takes its multiplications, a few additions over W lanes and no more.
+//   values: L lanes hold the row's elements, eight each, for 32 / L keys at a
+//     time, and the weights come from shared memory.
+// Chunks are swizzled (rows padded, where a row's chunks are no multiple of
+// eight) so that the keys of either pattern lie in different banks.  With FULL,
+// D is 8 L: known to the compiler, no lane idle.
 template <class T_, int L, int NH_, bool FULL>
 struct LaneTile {
   using T = T_;
   static constexpr int NH = NH_;
   static constexpr int kKeysAtOnce = 32 / L, kSteps = 4;
   static constexpr int TK = kSteps * kKeysAtOnce;  // keys of a warp's tile
-  // A stage holds K and V rows of at most TK * 8 L elements: 8 KB in fp32, 4 KB
-  // in 16 bits.  Two blocks of four warps on an SM then have about 128 KB on the way.
-  static constexpr int kStages = (NH <= 4 ? 2 : 3) * (sizeof(T) == 4 ? 1 : 2);
-  static constexpr int N = kSteps * NH;                   // scores of a lane before the exchange
-  static constexpr int E = N >= L ? N / L : 1;            // after it
-  static constexpr int kCopies = N >= L ? 1 : L / N;      // lanes that hold the same score
-  static constexpr int HE = E < NH ? E : NH;              // different heads among a lane's scores
-  // Floats a warp: each weight twice, as the operand of a multiplication of
-  // pairs, then a factor a head; in units of 16 bytes.
-  static constexpr int kScratch = 2 * TK * NH + (NH + 3) / 4 * 4;
+  static constexpr int W = 32 / TK;
+  // With two stages three blocks find room on an SM, with about 96 KB on the
+  // way; twelve warps hide each other's waits better than eight with a third stage (b64
+  // of 9/3 x 64 heads, fp32: 52 us with three stages, 37 with two).
+  static constexpr int kStages = (NH <= 6 ? 2 : 3) * (sizeof(T) == 4 ? 1 : 2);
+  static constexpr int kMinBlocks = NH <= 6 ? 3 : 2;  // of an SM: what the stages leave room for
+  static constexpr int kPer = 16 / sizeof(T);         // elements of a chunk
+  static constexpr int NP = NH == 1 ? 1 : (NH + 1) / 2 * 2;
+  // Floats a warp: each weight twice, as the operand of a multiplication of pairs.
+  static constexpr int kScratch = 2 * TK * NP;
   static constexpr int kD = FULL ? 8 * L : 0;
-  static constexpr int kMinBlocks = NH <= 4 ? 3 : 2;  // of an SM: what the stages leave room for
+  static constexpr bool kSharedQ = true;
   static_assert(2 * TK * sizeof(T) >= NH * 4, "a warp's state fits into a stage");
 
-  uint64_t q[NH][4], acc[NH][4];
-  float m[HE], l[HE];
-  int D, lane, l_id, group;
-  int key0, head0;  // of the first score that this lane holds after the exchange
+  uint64_t acc[NH][4];
+  float m[NH], l[NH];
+  int D, lane, l_id, group, vecs;
+  int qk_row, qk_xor, pv0, pv1;  // byte offsets into a tile's rows
   bool in0, in1;
 
-  __host__ __device__ static int row_bytes(int D) { return D * (int)sizeof(T); }
-  __device__ static __forceinline__ int chunk_at(int, int chunk) { return chunk; }
+  __host__ __device__ static __forceinline__ int row_bytes(int D) {
+    const int n = D * (int)sizeof(T);
+    if (n % 128 == 0) return n;
+    // a distance of 16 W or -16 W modulo 128 bytes puts the keys of eight lanes into different banks
+    const int up = (16 * W % 128 - n % 128 + 128) % 128, down = (128 - 16 * W % 128 - n % 128 + 256) % 128;
+    return n + (up < down ? up : down);
+  }
+  __device__ static __forceinline__ int swizzle(int row, int D) {
+    return D * (int)sizeof(T) % 128 == 0 ? row * W & 7 : 0;
+  }
+  __device__ static __forceinline__ int chunk_at(int row, int chunk, int D) { return chunk ^ swizzle(row, D); }
 
   __device__ __forceinline__ int elem(int i) const {  // element of slot i (0 .. 7) of this lane
     return sizeof(T) == 4 ? (i < 4 ? l_id * 4 + i : (l_id + L) * 4 + i - 4) : l_id * 8 + i;
   }
-  // Score e of this lane (step * NH + head counts them from n0): key and head.
-  __device__ __forceinline__ int key_of(int e) const { return key0 + e / NH * kKeysAtOnce; }
-  __device__ __forceinline__ int head_of(int e) const { return E < NH ? head0 + e : e % NH; }
 
-  template <class A>
-  __device__ __forceinline__ void load_q(const A* q0, int nh, float scale) {
-#pragma unroll
-    for (int g = 0; g < NH; ++g) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = g < nh && elem(i) < D ? to_f(q0[g * D + elem(i)]) * scale : 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        q[g][i] = pack2(x[2 * i], x[2 * i + 1]);
-        acc[g][i] = 0;
-      }
-    }
-  }
-
-  __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t b, int h0, int nh) {
+  __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t, int, int) {
     D = FULL ? 8 * L : p.geom.head_dim;
+    vecs = D / kPer;
     lane = threadIdx.x % 32;
     l_id = lane % L;
     group = lane / L;
-    const int n0 = N >= L ? l_id * E : l_id / kCopies;
-    key0 = n0 / NH * kKeysAtOnce + group;
-    head0 = n0 % NH;
-    const int vecs = D * (int)sizeof(T) / 16;
     in0 = FULL || l_id < vecs;
     in1 = FULL || l_id + L < vecs;
-    const int64_t at = b * p.q_stride + (int64_t)h0 * D;
-    if (p.dt == DT_F32) load_q(static_cast<const float*>(p.q) + at, nh, p.scale);
-    else if (p.dt == DT_F16) load_q(static_cast<const __half*>(p.q) + at, nh, p.scale);
-    else load_q(static_cast<const __nv_bfloat16*>(p.q) + at, nh, p.scale);
+    const int rb = row_bytes(D), key = lane / W;
+    qk_row = key * rb;
+    qk_xor = swizzle(key, D) * 16;
+    // the swizzle of row st * kKeysAtOnce + group does not depend on st: kKeysAtOnce * W is 8
+    pv0 = group * rb + chunk_at(group, l_id, D) * 16;
+    pv1 = group * rb + chunk_at(group, l_id + L, D) * 16;
 #pragma unroll
-    for (int e = 0; e < HE; ++e) {
-      m[e] = -INFINITY;
-      l[e] = 0.f;
+    for (int g = 0; g < NH; ++g) {
+      m[g] = -INFINITY;
+      l[g] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[g][i] = 0;
     }
   }
 
-  __device__ __forceinline__ void load_row(const char* row, uint64_t (&x)[4]) const {
+  // A chunk of a row as pairs of fp32 values.
+  __device__ static __forceinline__ void load_chunk(const char* at, uint64_t (&x)[kPer / 2]) {
     if constexpr (sizeof(T) == 4) {
-      const float4 a = in0 ? *reinterpret_cast<const float4*>(row + l_id * 16) : make_float4(0, 0, 0, 0);
-      const float4 c = in1 ? *reinterpret_cast<const float4*>(row + (l_id + L) * 16) : make_float4(0, 0, 0, 0);
-      x[0] = pack2(a.x, a.y);
-      x[1] = pack2(a.z, a.w);
-      x[2] = pack2(c.x, c.y);
-      x[3] = pack2(c.z, c.w);
+      const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(at);
+      x[0] = a.x;
+      x[1] = a.y;
     } else {
-      const uint4 a = in0 ? *reinterpret_cast<const uint4*>(row + l_id * 16) : make_uint4(0, 0, 0, 0);
+      const uint4 a = *reinterpret_cast<const uint4*>(at);
       const T* h = reinterpret_cast<const T*>(&a);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = pack2(to_f(h[2 * i]), to_f(h[2 * i + 1]));
     }
   }
 
-  // One tile: K and V rows of TK keys, `add` their mask values; `live` keys
-  // from the first are within the sequence.  Scores go to `scores` (nullptr:
-  // not wanted), [key][group size].
-  __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float* scratch, float* scores,
-                                       int live, int group_size, int nh) {
-    const int rb = row_bytes(D);
-    float s[N];
+  // One tile: K and V rows of TK keys, `add` their mask values, q the scaled
+  // queries [NH][D] in shared memory; `live` keys from the first are within
+  // the sequence.  Scores go to `scores` (nullptr: not wanted), [key][group size].
+  __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float* scratch, const float* q,
+                                       float* scores, int live, int group_size, int nh) {
+    const int rb = row_bytes(D), key = lane / W;
+    uint64_t dot[NH] = {};
+    const char* krow = ks + qk_row;
+    const float* qw = q + lane % W * kPer;
+    auto chunk = [&](int c0) {  // chunk c0 + lane % W
+      uint64_t x[kPer / 2];
+      load_chunk(krow + ((c0 + lane % W) * 16 ^ qk_xor), x);
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      uint64_t x[4];
-      load_row(ks + (st * kKeysAtOnce + group) * rb, x);
+      for (int g = 0; g < NH; ++g)
 #pragma unroll
-      for (int g = 0; g < NH; ++g) {
-        uint64_t d = mul2(q[g][0], x[0]);
+        for (int i = 0; i < kPer / 2; i += 2) {
+          const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(qw + g * D + c0 * kPer + 2 * i);
+          dot[g] = fma2(y.x, x[i], dot[g]);
+          dot[g] = fma2(y.y, x[i + 1], dot[g]);
+        }
+    };
+    if constexpr (FULL) {
 #pragma unroll
-        for (int i = 1; i < 4; ++i) d = fma2(q[g][i], x[i], d);
-        const float2 f = unpack2(d);
-        s[st * NH + g] = f.x + f.y;
-      }
+      for (int c0 = 0; c0 < 8 * L / kPer; c0 += W) chunk(c0);
+    } else {
+      for (int c0 = 0; c0 < vecs; c0 += W)
+        if (c0 + lane % W < vecs) chunk(c0);
     }
-    // sums over the L lanes, halving what a lane holds
-    int cnt = N;
-#pragma unroll
-    for (int o = L / 2; o; o >>= 1) {
-      const bool upper = lane & o;
-      if (cnt > 1) {
-        cnt >>= 1;
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i)
-          if (i < cnt) {
-            const float send = upper ? s[i] : s[i + cnt], keep = upper ? s[i + cnt] : s[i];
-            s[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-          }
-      } else {
-        s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
-      }
-    }
-    float mx[HE];
-#pragma unroll
-    for (int e = 0; e < HE; ++e) mx[e] = m[e];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      s[e] += add[key_of(e)];
-      mx[e % HE] = fmaxf(mx[e % HE], s[e]);
-    }
-    if (scores) {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (key_of(e) < live && head_of(e) < nh) scores[key_of(e) * group_size + head_of(e)] = s[e];
-    }
-    // the maximum over the lanes that hold other keys of the same heads
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-      if (o >= L || (o >= kCopies && o * E / kCopies >= NH))
-#pragma unroll
-        for (int e = 0; e < HE; ++e) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
+    float s[NH];
+    const float a = add[key];
     bool changed = false;
+    float mx[NH];
 #pragma unroll
-    for (int e = 0; e < HE; ++e) changed |= mx[e] != m[e];
-    if (__any_sync(0xffffffffu, changed)) {
-      float* c = scratch + 2 * TK * NH;
+    for (int g = 0; g < NH; ++g) {
+      const float2 f = unpack2(dot[g]);
+      s[g] = f.x + f.y;
 #pragma unroll
-      for (int e = 0; e < HE; ++e) {
-        const float f = exp_from(m[e], mx[e]);
-        l[e] *= f;
-        m[e] = mx[e];
-        c[head_of(e)] = f;
-      }
-      __syncwarp();
+      for (int o = W / 2; o; o >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
+      s[g] += a;
+      mx[g] = fmaxf(m[g], warp_max(s[g]));
+      changed |= mx[g] != m[g];
+    }
+    if (scores && lane % W == 0 && key < live) {
+#pragma unroll
+      for (int g = 0; g < NH; ++g)
+        if (g < nh) scores[key * group_size + g] = s[g];
+    }
+    if (changed) {  // the same for all lanes
 #pragma unroll
       for (int g = 0; g < NH; ++g) {
-        const uint64_t f = pack2(c[g], c[g]);
+        const float c = exp_from(m[g], mx[g]);
+        m[g] = mx[g];
+        l[g] *= c;
+        const uint64_t f = pack2(c, c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[g][i] = mul2(acc[g][i], f);
       }
     }
     uint64_t* pairs = reinterpret_cast<uint64_t*>(scratch);
+    uint64_t w[NP];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float x = exp_from(s[e], m[e % HE]);
-      l[e % HE] += x;
-      pairs[key_of(e) * NH + head_of(e)] = pack2(x, x);
+    for (int g = 0; g < NP; ++g) w[g] = 0;
+#pragma unroll
+    for (int g = 0; g < NH; ++g) {
+      const float x = exp_from(s[g], m[g]);
+      l[g] += x;
+      w[g] = pack2(x, x);
+    }
+    if (lane % W == 0) {
+      if constexpr (NH == 1) {
+        pairs[key] = w[0];
+      } else {
+#pragma unroll
+        for (int g = 0; g < NP; g += 2)
+          *reinterpret_cast<ulonglong2*>(pairs + key * NP + g) = make_ulonglong2(w[g], w[g + 1]);
+      }
     }
     __syncwarp();
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
-      const int key = st * kKeysAtOnce + group;
-      uint64_t x[4], f[NH];
-      load_row(vs + key * rb, x);
+      const int at = st * kKeysAtOnce * rb;
+      uint64_t x[4];
+      if constexpr (sizeof(T) == 4) {
+        uint64_t h[2];
+        load_chunk(vs + at + (in0 ? pv0 : 0), h);
+        x[0] = in0 ? h[0] : 0;
+        x[1] = in0 ? h[1] : 0;
+        load_chunk(vs + at + (in1 ? pv1 : 0), h);
+        x[2] = in1 ? h[0] : 0;
+        x[3] = in1 ? h[1] : 0;
+      } else {
+        load_chunk(vs + at + (in0 ? pv0 : 0), x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = in0 ? x[i] : 0;
+      }
+      const uint64_t* row = pairs + (st * kKeysAtOnce + group) * NP;
+      uint64_t f[NP];
       if constexpr (NH == 1) {
-        f[0] = pairs[key];
+        f[0] = row[0];
       } else {
 #pragma unroll
-        for (int g = 0; g < NH; g += 2) {
-          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(pairs + key * NH + g);
+        for (int g = 0; g < NP; g += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(row + g);
           f[g] = two.x;
           f[g + 1] = two.y;
         }
@@ -285,17 +292,14 @@ struct LaneTile {
   // The warp's state: ml[2 * head] the maximum, ml[2 * head + 1] the sum, o[head * D + d].
   __device__ __forceinline__ void dump(float* ml, float* o) {
 #pragma unroll
-    for (int off = 16; off; off >>= 1)
-      if (off >= L || (off >= kCopies && off * E / kCopies >= NH))
-#pragma unroll
-        for (int e = 0; e < HE; ++e) l[e] += __shfl_xor_sync(0xffffffffu, l[e], off);
-#pragma unroll
-    for (int e = 0; e < HE; ++e) {
-      ml[2 * head_of(e)] = m[e];
-      ml[2 * head_of(e) + 1] = l[e];
-    }
-#pragma unroll
     for (int g = 0; g < NH; ++g) {
+      float sum = lane % W == 0 ? l[g] : 0.f;  // each key once
+#pragma unroll
+      for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (lane == 0) {
+        ml[2 * g] = m[g];
+        ml[2 * g + 1] = sum;
+      }
       float x[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -309,8 +313,9 @@ struct LaneTile {
         for (int i = 0; i < 8; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], off);
       if (group == 0)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (elem(i) < D) o[g * D + elem(i)] = x[i];
+        for (int i = 0; i < 8; i += 4)
+          if (elem(i) < D)
+            *reinterpret_cast<float4*>(o + g * D + elem(i)) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
     }
   }
 };
@@ -332,6 +337,7 @@ struct MmaTile {
   static constexpr int TK = DT == 64 ? 32 : 16;
   static constexpr int kStages = 3;
   static constexpr int kScratch = 0;
+  static constexpr bool kSharedQ = false;
   static constexpr int kD = FULL ? DT : 0;
   static constexpr int R = NH / 8;  // head rows of a thread
   static constexpr int kMinBlocks = DT == 256 ? 1 : 2;
@@ -344,7 +350,7 @@ struct MmaTile {
   int D, lane;
 
   __host__ __device__ static int row_bytes(int) { return DT * 2; }
-  __device__ static __forceinline__ int chunk_at(int row, int chunk) { return chunk ^ (row & 7); }
+  __device__ static __forceinline__ int chunk_at(int row, int chunk, int = 0) { return chunk ^ (row & 7); }
 
   __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t b, int h0, int nh) {
     D = FULL ? DT : p.geom.head_dim;
@@ -407,8 +413,8 @@ struct MmaTile {
     lo = *reinterpret_cast<uint32_t*>(r);
   }
 
-  __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float*, float* scores, int live,
-                                       int group_size, int nh) {
+  __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float*, const float*, float* scores,
+                                       int live, int group_size, int nh) {
     constexpr int RB = DT * 2;
     const uint32_t kb = smem_u32(ks), vb = smem_u32(vs);
     float s[TK / 8][4];
@@ -553,15 +559,16 @@ __device__ __forceinline__ int units_of(int len) {
   return len < 0 ? 0 : tiles_of<TILE>(len) + kStart;
 }
 
-// Shared memory in bytes: the warps' stages, their mask values and scratch.  At
+// Shared memory in bytes: the warps' stages, their mask values and scratch, and the queries.  At
 // the end of a segment a warp's state takes the place of the stage that it has just
 // used, which the next tile's load fills again: in all types NH * D floats fit
 // into the 2 * TK rows of a stage.
 template <class P>
 __host__ __device__ constexpr int attend_stage_bytes(int row_bytes) { return 2 * P::TK * row_bytes; }
 template <class P>
-inline int attend_smem(int row_bytes) {
-  return kWarps * (P::kStages * (attend_stage_bytes<P>(row_bytes) + P::TK * 4) + P::kScratch * 4);
+inline int attend_smem(int row_bytes, int D) {
+  return kWarps * (P::kStages * (attend_stage_bytes<P>(row_bytes) + P::TK * 4) + P::kScratch * 4) +
+         (P::kSharedQ ? P::NH * D * 4 : 0);
 }
 
 template <class P>
@@ -674,8 +681,17 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   char* ring = smem + warp * NS * stage_bytes;
   float* adds = reinterpret_cast<float*>(smem + kWarps * NS * stage_bytes) + warp * NS * TK;
   float* scratch = reinterpret_cast<float*>(smem + kWarps * NS * (stage_bytes + TK * 4)) + warp * P::kScratch;
+  // The segment's queries, scaled, [NH][D]: the block fetches the next ones while it joins a segment.
+  float* queries = reinterpret_cast<float*>(smem + kWarps * (NS * (stage_bytes + TK * 4) + P::kScratch * 4));
+  auto fetch_q = [&](const Cursor& c) {
+    if constexpr (P::kSharedQ) {
+      const int h = c.kvh * group + c.chunk * NH, n = min(NH, group - c.chunk * NH) * D;
+      const int64_t at = c.b * p.q_stride + (int64_t)h * D;
+      for (int x = tid; x < n; x += kThreads) queries[x] = load_act(p.q, p.dt, at + x) * p.scale;
+    }
+  };
   // Tensor cores read the padding of K rows up to DT, against zeros of q: it holds zeros, which no load overwrites.
-  const bool padded = !P::kD && rb != D * (int)sizeof(T);
+  const bool padded = !P::kD && !P::kSharedQ && rb != D * (int)sizeof(T);
   auto clear = [&](char* at, int bytes) {
     for (int i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
     __syncwarp();
@@ -734,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
           for (int v = 0; v < TK * V; v += 32) {
             const int row = V <= 32 ? v / V + lane / V : v / V, col = V <= 32 ? lane % V : v % V + lane;
             const char* src = from + __shfl_sync(0xffffffffu, off, row) + (V <= 32 ? 0 : v % V * 16);
-            const int s = row * rb + P::chunk_at(row, col) * 16;
+            const int s = row * rb + P::chunk_at(row, col, D) * 16;
             copy16(ka + s, src);
             copy16(va + s, src + to_v);
           }
@@ -743,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
 #pragma unroll 4
           for (int v = 0; v < TK * vecs; v += 32) {
             const char* src = from + __shfl_sync(0xffffffffu, off, row & 31) + col * 16;
-            const int s = row * rb + P::chunk_at(row, col) * 16;
+            const int s = row * rb + P::chunk_at(row, col, D) * 16;
             if (row < TK) {
               copy16(ka + s, src);
               copy16(va + s, src + to_v);
@@ -767,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         if (row < TK && !(put_new && row == new_row)) {
           const bool ok = o >= 0;
           const long long at = ok ? o + col * 16 : 0;
-          const int s = row * rb + P::chunk_at(row, col) * 16;
+          const int s = row * rb + P::chunk_at(row, col, D) * 16;
           copy16(smem_u32(ks + s), static_cast<const char*>(p.k_pages) + at, ok);
           copy16(smem_u32(vs + s), static_cast<const char*>(p.v_pages) + at, ok);
         }
@@ -785,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
           const T k = from_f<T>(load_act(p.k, p.dt, c.b * p.k_stride + c.kvh * D + d));
           const T v = from_f<T>(load_act(p.v, p.dt, c.b * p.v_stride + c.kvh * D + d));
           if (put_new) {
-            const int s = new_row * rb + P::chunk_at(new_row, d * (int)sizeof(T) / 16) * 16 + d * (int)sizeof(T) % 16;
+            const int s = new_row * rb + P::chunk_at(new_row, d * (int)sizeof(T) / 16, D) * 16 + d * (int)sizeof(T) % 16;
             *reinterpret_cast<T*>(ks + s) = k;
             *reinterpret_cast<T*>(vs + s) = v;
           }
@@ -813,6 +829,12 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     copy_commit();
   }
 
+  if (P::kSharedQ) {
+    for (int x = tid; x < NH * D; x += kThreads) queries[x] = 0.f;  // heads that the last chunk has not
+    __syncthreads();
+    fetch_q(use);
+    __syncthreads();
+  }
   int stage = 0, load_stage = NS - 1;  // of the tile in use, and of the next tile to load
   int j = 0;
 #pragma unroll 1
@@ -843,8 +865,8 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         load_stage = load_stage + 1 == NS ? 0 : load_stage + 1;
         stage_at = stage * stage_bytes;
         if (first < use.len)
-          state.tile(ring + stage_at, ring + stage_at + TK * rb, adds + stage * TK, scratch, scores, use.len - first, group,
-                     nh);
+          state.tile(ring + stage_at, ring + stage_at + TK * rb, adds + stage * TK, scratch, queries, scores,
+                     use.len - first, group, nh);
         stage = stage + 1 == NS ? 0 : stage + 1;
         first += TILE;
         if (p.weights_out) scores += (long long)TILE * group;
@@ -857,6 +879,11 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     {
       // join the warps
       __syncthreads();
+      if (j < count) {
+        Cursor next = use;
+        advance(next);
+        fetch_q(next);
+      }
       const bool begins = own_begin, whole = begins && seg_end;
       const int dv = D / 4;  // the results are taken four at a time
       // A part in the workspace: [NH][2], padded to 16 bytes, then [nh][D], counted
@@ -919,7 +946,7 @@ cudaError_t blocks_per_sm(int device, int smem, int* out) {
 
 template <class P>
 cudaError_t attend_launch(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
-  const int D = p.geom.head_dim, smem = attend_smem<P>(P::row_bytes(D));
+  const int D = p.geom.head_dim, smem = attend_smem<P>(P::row_bytes(D), D);
   int per_sm = 0;
   if (cudaError_t e = blocks_per_sm<P>(p.device, smem, &per_sm)) return e;
   shape->heads = P::NH;
@@ -928,16 +955,22 @@ cudaError_t attend_launch(const KvAttendParams& p, KvAttendShape* shape, cudaStr
   return cudaGetLastError();
 }
 
-// The kernel for these types, head dim and group.
+// The kernel for these types, head dim and group: a group of more than eight
+// heads (four, where a stage of four 16-bit rows holds the states of no more)
+// is divided evenly.
 template <class T, int L, bool FULL>
 cudaError_t attend_lanes_group(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
-  const int group = p.heads / p.geom.kv_heads;
-  if (group <= 1) return attend_launch<LaneTile<T, L, 1, FULL>>(p, shape, s);
-  if (group <= 2) return attend_launch<LaneTile<T, L, 2, FULL>>(p, shape, s);
-  // a stage of four 16-bit rows has no room for the states of eight heads
   constexpr int kMost = L == 32 && sizeof(T) == 2 ? 4 : 8;
-  if (group <= 4) return attend_launch<LaneTile<T, L, 4, FULL>>(p, shape, s);
-  return attend_launch<LaneTile<T, L, kMost, FULL>>(p, shape, s);
+  const int group = p.heads / p.geom.kv_heads, chunks = (group + kMost - 1) / kMost, heads = (group + chunks - 1) / chunks;
+  if (heads <= 1) return attend_launch<LaneTile<T, L, 1, FULL>>(p, shape, s);
+  if (heads <= 2) return attend_launch<LaneTile<T, L, 2, FULL>>(p, shape, s);
+  if (heads <= 3) return attend_launch<LaneTile<T, L, 3, FULL>>(p, shape, s);
+  if (heads <= 4) return attend_launch<LaneTile<T, L, 4, FULL>>(p, shape, s);
+  if constexpr (kMost == 8) {
+    if (heads <= 6) return attend_launch<LaneTile<T, L, 6, FULL>>(p, shape, s);
+    return attend_launch<LaneTile<T, L, 8, FULL>>(p, shape, s);
+  }
+  return cudaErrorInvalidValue;
 }
 template <class T>
 cudaError_t attend_lanes(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
