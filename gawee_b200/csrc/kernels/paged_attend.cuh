@@ -88,7 +88,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 //
 // Lanes: any types, all products in fp32, two to an instruction.  A warp's tile
 // has TK = 128 / L keys of D <= 8 L elements: 8 KB of K and V in fp32, 4 KB in 16 bits.
-//   scores: W = L / 4 lanes share a key and take every W-th 16-byte chunk of its
+//   scores: W lanes share a key (or two) and take every W-th 16-byte chunk of its
 //     row; the query heads come from shared memory, the same address for all
 //     keys, so that a score takes its multiplications, a few additions over W lanes and no more.
 //   values: L lanes hold the row's elements, eight each, for 32 / L keys at a
@@ -102,7 +102,12 @@ struct LaneTile {
   static constexpr int NH = NH_;
   static constexpr int kKeysAtOnce = 32 / L, kSteps = 4;
   static constexpr int TK = kSteps * kKeysAtOnce;  // keys of a warp's tile
-  static constexpr int W = 32 / TK;
+  // Lanes that share a key, and the keys that they take at once: two for long
+  // fp32 rows and several heads, where the reads of the queries would fill shared
+  // memory's time (8 heads x 128, 74,862 rows: 74 us, with one key 84; in 16 bits
+  // with 4 heads one key is the faster, 51 against 52).
+  static constexpr int KL = sizeof(T) == 4 && L >= 16 && NH >= 4 ? 2 : 1;
+  static constexpr int W = 32 * KL / TK, kOwn = W / KL;  // kOwn lanes end up with the same key
   // With two stages three blocks find room on an SM, with about 96 KB on the
   // way; twelve warps hide each other's waits better than eight with a third stage (b64
   // of 9/3 x 64 heads, fp32: 52 us with three stages, 37 with two).
@@ -119,12 +124,13 @@ struct LaneTile {
   uint64_t acc[NH][4];
   float m[NH], l[NH];
   int D, lane, l_id, group, vecs;
+  int own_key;                   // of the scores that this lane ends up with
   int qk_row, qk_xor, pv0, pv1;  // byte offsets into a tile's rows
   bool in0, in1;
 
   __host__ __device__ static __forceinline__ int row_bytes(int D) {
     const int n = D * (int)sizeof(T);
-    if (n % 128 == 0) return n;
+    if (n % 128 == 0 || W >= 8) return n;  // eight lanes read consecutive chunks of one row, or of swizzled ones
     // a distance of 16 W or -16 W modulo 128 bytes puts the keys of eight lanes into different banks
     const int up = (16 * W % 128 - n % 128 + 128) % 128, down = (128 - 16 * W % 128 - n % 128 + 256) % 128;
     return n + (up < down ? up : down);
@@ -149,7 +155,8 @@ struct LaneTile {
     const int rb = row_bytes(D), key = lane / W;
     qk_row = key * rb;
     qk_xor = swizzle(key, D) * 16;
-    // the swizzle of row st * kKeysAtOnce + group does not depend on st: kKeysAtOnce * W is 8
+    own_key = key + (KL == 2 && (lane & W / 2) ? TK / 2 : 0);
+    // the swizzle of row st * kKeysAtOnce + group does not depend on st: kKeysAtOnce * W is a multiple of 8
     pv0 = group * rb + chunk_at(group, l_id, D) * 16;
     pv1 = group * rb + chunk_at(group, l_id + L, D) * 16;
 #pragma unroll
@@ -180,20 +187,24 @@ struct LaneTile {
   // the sequence.  Scores go to `scores` (nullptr: not wanted), [key][group size].
   __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float* scratch, const float* q,
                                        float* scores, int live, int group_size, int nh) {
-    const int rb = row_bytes(D), key = lane / W;
-    uint64_t dot[NH] = {};
-    const char* krow = ks + qk_row;
+    const int rb = row_bytes(D), key = own_key;
+    uint64_t dot[KL][NH] = {};
+    const char* krow = ks + qk_row;  // and, with two keys, TK / 2 rows on (the same swizzle: W is then 8 or more)
     const float* qw = q + lane % W * kPer;
     auto chunk = [&](int c0) {  // chunk c0 + lane % W
-      uint64_t x[kPer / 2];
-      load_chunk(krow + ((c0 + lane % W) * 16 ^ qk_xor), x);
+      uint64_t x[KL][kPer / 2];
+#pragma unroll
+      for (int u = 0; u < KL; ++u) load_chunk(krow + u * (TK / 2) * rb + ((c0 + lane % W) * 16 ^ qk_xor), x[u]);
 #pragma unroll
       for (int g = 0; g < NH; ++g)
 #pragma unroll
         for (int i = 0; i < kPer / 2; i += 2) {
           const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(qw + g * D + c0 * kPer + 2 * i);
-          dot[g] = fma2(y.x, x[i], dot[g]);
-          dot[g] = fma2(y.y, x[i + 1], dot[g]);
+#pragma unroll
+          for (int u = 0; u < KL; ++u) {
+            dot[u][g] = fma2(y.x, x[u][i], dot[u][g]);
+            dot[u][g] = fma2(y.y, x[u][i + 1], dot[u][g]);
+          }
         }
     };
     if constexpr (FULL) {
@@ -209,15 +220,21 @@ struct LaneTile {
     float mx[NH];
 #pragma unroll
     for (int g = 0; g < NH; ++g) {
-      const float2 f = unpack2(dot[g]);
+      const float2 f = unpack2(dot[0][g]);
       s[g] = f.x + f.y;
+      if constexpr (KL == 2) {  // the upper half of the lanes keeps the second key
+        const float2 f1 = unpack2(dot[1][g]);
+        const float s1 = f1.x + f1.y;
+        const bool upper = lane & W / 2;
+        s[g] = (upper ? s1 : s[g]) + __shfl_xor_sync(0xffffffffu, upper ? s[g] : s1, W / 2);
+      }
 #pragma unroll
-      for (int o = W / 2; o; o >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
+      for (int o = kOwn / 2; o; o >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
       s[g] += a;
       mx[g] = fmaxf(m[g], warp_max(s[g]));
       changed |= mx[g] != m[g];
     }
-    if (scores && lane % W == 0 && key < live) {
+    if (scores && lane % kOwn == 0 && key < live) {
 #pragma unroll
       for (int g = 0; g < NH; ++g)
         if (g < nh) scores[key * group_size + g] = s[g];
@@ -243,7 +260,7 @@ struct LaneTile {
       l[g] += x;
       w[g] = pack2(x, x);
     }
-    if (lane % W == 0) {
+    if (lane % kOwn == 0) {
       if constexpr (NH == 1) {
         pairs[key] = w[0];
       } else {
@@ -293,7 +310,7 @@ struct LaneTile {
   __device__ __forceinline__ void dump(float* ml, float* o) {
 #pragma unroll
     for (int g = 0; g < NH; ++g) {
-      float sum = lane % W == 0 ? l[g] : 0.f;  // each key once
+      float sum = lane % kOwn == 0 ? l[g] : 0.f;  // each key once
 #pragma unroll
       for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
       if (lane == 0) {
