@@ -118,7 +118,8 @@ struct LaneTile {
   // Floats a warp: each weight twice, as the operand of a multiplication of pairs.
   static constexpr int kScratch = 2 * TK * NP;
   static constexpr int kD = FULL ? 8 * L : 0;
-  static constexpr bool kSharedQ = true;
+  using Query = float;                        // in shared memory: scaled
+  static constexpr int kMaxD = 8 * L, kQueryPad = 0;
   static_assert(2 * TK * sizeof(T) >= NH * 4, "a warp's state fits into a stage");
 
   uint64_t acc[NH][4];
@@ -144,7 +145,10 @@ struct LaneTile {
     return sizeof(T) == 4 ? (i < 4 ? l_id * 4 + i : (l_id + L) * 4 + i - 4) : l_id * 8 + i;
   }
 
-  __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t, int, int) {
+  __device__ static __forceinline__ float query(const void* q, int dt, int64_t i, float scale) {
+    return load_act(q, dt, i) * scale;
+  }
+  __device__ __forceinline__ void begin(const KvAttendParams& p, const float*, int) {
     D = FULL ? 8 * L : p.geom.head_dim;
     vecs = D / kPer;
     lane = threadIdx.x % 32;
@@ -354,7 +358,8 @@ struct MmaTile {
   static constexpr int TK = DT == 64 ? 32 : 16;
   static constexpr int kStages = 3;
   static constexpr int kScratch = 0;
-  static constexpr bool kSharedQ = false;
+  using Query = T;  // in shared memory, rows 16 bytes further apart: eight heads lie in different banks
+  static constexpr int kMaxD = DT, kQueryPad = 8;
   static constexpr int kD = FULL ? DT : 0;
   static constexpr int R = NH / 8;  // head rows of a thread
   static constexpr int kMinBlocks = DT == 256 ? 1 : 2;
@@ -369,11 +374,11 @@ struct MmaTile {
   __host__ __device__ static int row_bytes(int) { return DT * 2; }
   __device__ static __forceinline__ int chunk_at(int row, int chunk, int = 0) { return chunk ^ (row & 7); }
 
-  __device__ __forceinline__ void begin(const KvAttendParams& p, int64_t b, int h0, int nh) {
+  __device__ static __forceinline__ T query(const void* q, int, int64_t i, float) { return static_cast<const T*>(q)[i]; }
+  __device__ __forceinline__ void begin(const KvAttendParams& p, const T* queries, int nh) {
     D = FULL ? DT : p.geom.head_dim;
     lane = threadIdx.x % 32;
     scale = p.scale;
-    const T* base = static_cast<const T*>(p.q) + b * p.q_stride + (int64_t)h0 * D;
 #pragma unroll
     for (int k = 0; k < DT / 16; ++k)
 #pragma unroll
@@ -381,12 +386,8 @@ struct MmaTile {
         // registers of A: rows g (and g + 8), columns 2c, 2c + 1 (and + 8)
         const int head = lane / 4 + (R == 2 ? (i & 1) * 8 : 0);
         const int d = k * 16 + lane % 4 * 2 + (R == 2 ? i >> 1 : i) * 8;
-        T x[2] = {from_f<T>(0.f), from_f<T>(0.f)};
-        if (head < nh && d < D) {  // D is even
-          x[0] = base[(int64_t)head * D + d];
-          x[1] = base[(int64_t)head * D + d + 1];
-        }
-        q[k][i] = *reinterpret_cast<uint32_t*>(x);
+        const bool in = head < nh && d < D;  // D is even
+        q[k][i] = in ? *reinterpret_cast<const uint32_t*>(queries + head * (D + kQueryPad) + d) : 0u;
       }
 #pragma unroll
     for (int j = 0; j < DT / 8; ++j)
@@ -430,7 +431,7 @@ struct MmaTile {
     lo = *reinterpret_cast<uint32_t*>(r);
   }
 
-  __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float*, const float*, float* scores,
+  __device__ __forceinline__ void tile(const char* ks, const char* vs, const float* add, float*, const T*, float* scores,
                                        int live, int group_size, int nh) {
     constexpr int RB = DT * 2;
     const uint32_t kb = smem_u32(ks), vb = smem_u32(vs);
@@ -585,7 +586,7 @@ __host__ __device__ constexpr int attend_stage_bytes(int row_bytes) { return 2 *
 template <class P>
 inline int attend_smem(int row_bytes, int D) {
   return kWarps * (P::kStages * (attend_stage_bytes<P>(row_bytes) + P::TK * 4) + P::kScratch * 4) +
-         (P::kSharedQ ? P::NH * D * 4 : 0);
+         P::NH * (D + P::kQueryPad) * (int)sizeof(typename P::Query);
 }
 
 template <class P>
@@ -698,17 +699,30 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   char* ring = smem + warp * NS * stage_bytes;
   float* adds = reinterpret_cast<float*>(smem + kWarps * NS * stage_bytes) + warp * NS * TK;
   float* scratch = reinterpret_cast<float*>(smem + kWarps * NS * (stage_bytes + TK * 4)) + warp * P::kScratch;
-  // The segment's queries, scaled, [NH][D]: the block fetches the next ones while it joins a segment.
-  float* queries = reinterpret_cast<float*>(smem + kWarps * (NS * (stage_bytes + TK * 4) + P::kScratch * 4));
+  // The segment's queries, [NH][D]: fetched into registers while the last
+  // segment is joined, then put into shared memory.
+  using Query = typename P::Query;
+  constexpr int kQueryEach = (NH * P::kMaxD + kThreads - 1) / kThreads;
+  Query* queries = reinterpret_cast<Query*>(smem + kWarps * (NS * (stage_bytes + TK * 4) + P::kScratch * 4));
+  Query fetched[kQueryEach];
   auto fetch_q = [&](const Cursor& c) {
-    if constexpr (P::kSharedQ) {
-      const int h = c.kvh * group + c.chunk * NH, n = min(NH, group - c.chunk * NH) * D;
-      const int64_t at = c.b * p.q_stride + (int64_t)h * D;
-      for (int x = tid; x < n; x += kThreads) queries[x] = load_act(p.q, p.dt, at + x) * p.scale;
+    const int h = c.kvh * group + c.chunk * NH, n = min(NH, group - c.chunk * NH) * D;
+    const int64_t at = c.b * p.q_stride + (int64_t)h * D;
+#pragma unroll
+    for (int r = 0; r < kQueryEach; ++r) {
+      const int x = r * kThreads + tid;
+      fetched[r] = x < n ? P::query(p.q, p.dt, at + x, p.scale) : from_f<Query>(0.f);
+    }
+  };
+  auto put_q = [&] {
+#pragma unroll
+    for (int r = 0; r < kQueryEach; ++r) {
+      const int x = r * kThreads + tid;
+      if (x < NH * D) queries[P::kQueryPad ? x + x / D * P::kQueryPad : x] = fetched[r];
     }
   };
   // Tensor cores read the padding of K rows up to DT, against zeros of q: it holds zeros, which no load overwrites.
-  const bool padded = !P::kD && !P::kSharedQ && rb != D * (int)sizeof(T);
+  const bool padded = !P::kD && P::kScratch == 0 && rb != D * (int)sizeof(T);
   auto clear = [&](char* at, int bytes) {
     for (int i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
     __syncwarp();
@@ -834,6 +848,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   // fill the ring
   int issued = 0;
   fetch(load);
+  fetch_q(use);
 #pragma unroll 1
   for (; issued < NS - 1; ++issued) {
     if (issued < count) {
@@ -846,12 +861,8 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     copy_commit();
   }
 
-  if (P::kSharedQ) {
-    for (int x = tid; x < NH * D; x += kThreads) queries[x] = 0.f;  // heads that the last chunk has not
-    __syncthreads();
-    fetch_q(use);
-    __syncthreads();
-  }
+  put_q();
+  __syncthreads();
   int stage = 0, load_stage = NS - 1;  // of the tile in use, and of the next tile to load
   int j = 0;
 #pragma unroll 1
@@ -862,7 +873,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     int stage_at = 0;
     {
       P state;
-      state.begin(p, use.b, h0, nh);
+      state.begin(p, queries, nh);
       int first = use.tile * TILE + warp * TK;
       float* scores = nullptr;
       if (p.weights_out)
@@ -930,7 +941,8 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         const int last = (int)(((seg_begin + use.tiles + kStart) * blocks - 1) / total);
         p.info[((int64_t)use.b * kv + use.kvh) * chunks + use.chunk] = make_int2(blockIdx.x, last - (int)blockIdx.x + 1);
       }
-      __syncthreads();  // the stages are free again
+      if (j < count) put_q();
+      __syncthreads();  // the stages are free again, and the next queries there
       if (padded) clear(ring + stage_at, stage_bytes);
       seg_begin += use.tiles + kStart;
     }
