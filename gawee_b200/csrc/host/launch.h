@@ -35,7 +35,7 @@ Fn gather(const View& data, const View& idx, const View& out, int64_t pre, int64
 Fn gather_elements(const View& data, const View& idx, const View& out, int axis);
 Fn range(kern::RangeParams rp, const View& out);
 // One new token's attention over a paged key/value cache held in two arguments (kern::KvAttendParams):
-// q [B, H, D], k / v [B, Hkv, D], out dense; parts and info as kern::kv_parts_floats and kv_segments size them
+// q [B, H, D], k / v [B, Hkv, D], out dense; parts and info as kern::kv_parts_floats, kv_segments and kv_blocks size them
 Fn paged_attention(const View& q, const View& k, const View& v, const View& k_pages, const View& v_pages,
                    const View& table, const View& lengths, const View& out, const View& parts, const View& info,
                    float scale);

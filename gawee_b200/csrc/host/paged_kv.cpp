@@ -24,6 +24,7 @@ struct gawee_kv {
   float* scores = nullptr;     // [max_batch][heads][max_pages * page_size], with desc.weights
   float* parts = nullptr;      // attend's partial states
   int2* info = nullptr;        // attend's segments and the blocks that share them
+  int2* splits = nullptr;      // .. and its blocks and the segments that they leave unfinished
   int sms = 0;
   ~gawee_kv() {
     cudaFree(status);
@@ -32,6 +33,7 @@ struct gawee_kv {
     cudaFree(scores);
     cudaFree(parts);
     cudaFree(info);
+    cudaFree(splits);
   }
 };
 
@@ -172,6 +174,7 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     if (e == cudaSuccess)
       e = cudaMalloc((void**)&kv->info,
                      sizeof(int2) * gawee::kern::kv_segments(d.max_batch, d.kv_heads, d.heads / d.kv_heads));
+    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->splits, sizeof(int2) * gawee::kern::kv_blocks(kv->sms));
     if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
@@ -309,6 +312,7 @@ gawee_status gawee_kv_attend(gawee_kv* kv, const gawee_kv_attend_args* a, void* 
     p.stats = kv->stats;
     p.parts = kv->parts;
     p.info = kv->info;
+    p.splits = kv->splits;
     p.device = kv->device;
     p.sms = kv->sms;
     p.page_shift = gawee::kern::page_shift_of(kv->geom.page_size);

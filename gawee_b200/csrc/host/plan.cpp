@@ -1904,7 +1904,7 @@ class Planner {
     View out = alloc(DType::F32, val(n.outs[0]).type.shape);
     if (out.shape != q.shape) unsupported("paged_attention: the result has q's shape");
     View parts = alloc(DType::F32, {kern::kv_parts_floats(kern::kKvPlanSms, (int)(H / KV), (int)D)});
-    View info = alloc(DType::I32, {2 * kern::kv_segments(B, (int)KV, (int)(H / KV))});
+    View info = alloc(DType::I32, {2 * (kern::kv_segments(B, (int)KV, (int)(H / KV)) + kern::kv_blocks(kern::kKvPlanSms))});
     Op op;
     op.kind = OpKind::PAGED_ATTN;
     op.name = "paged_attention";

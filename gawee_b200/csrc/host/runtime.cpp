@@ -1052,6 +1052,7 @@ Fn paged_attention(const View& q, const View& k, const View& v, const View& k_pa
     p.out = rt.ptr(out);
     p.parts = reinterpret_cast<float*>(rt.ptr(parts));
     p.info = reinterpret_cast<int2*>(rt.ptr(info));
+    p.splits = p.info + kern::kv_segments(p.batch, p.geom.kv_heads, p.heads / p.geom.kv_heads);
     p.status = rt.status();
     p.device = rt.device;
     if (!p.sms) GCHECK(cudaDeviceGetAttribute(&p.sms, cudaDevAttrMultiProcessorCount, rt.device));

@@ -599,6 +599,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   __shared__ float s_ml[kWarps][NH][2];  // the warps' maxima and sums
   asm volatile("griddepcontrol.launch_dependents;");  // the join may take its place early: it waits for this grid's end
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  if (tid == 0) p.splits[blockIdx.x] = make_int2(0, 0);
   const int D = P::kD ? P::kD : p.geom.head_dim, kv = p.geom.kv_heads, group = p.heads / kv, chunks = (group + NH - 1) / NH;
   const int per_tile = kv * chunks;  // segments of a sequence
 
@@ -939,7 +940,9 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         // for the join: the segment's first block and the number of its blocks; the
         // block that holds unit u is the largest i with floor(total * i / blocks) <= u
         const int last = (int)(((seg_begin + use.tiles + kStart) * blocks - 1) / total);
-        p.info[((int64_t)use.b * kv + use.kvh) * chunks + use.chunk] = make_int2(blockIdx.x, last - (int)blockIdx.x + 1);
+        const int segment = (use.b * kv + use.kvh) * chunks + use.chunk, n = last - (int)blockIdx.x + 1;
+        p.info[segment] = make_int2(blockIdx.x, n);
+        if (n > 1) p.splits[blockIdx.x] = make_int2(segment, n);
       }
       if (j < count) put_q();
       __syncthreads();  // the stages are free again, and the next queries there
@@ -978,9 +981,10 @@ cudaError_t attend_launch(const KvAttendParams& p, KvAttendShape* shape, cudaStr
   const int D = p.geom.head_dim, smem = attend_smem<P>(P::row_bytes(D), D);
   int per_sm = 0;
   if (cudaError_t e = blocks_per_sm<P>(p.device, smem, &per_sm)) return e;
+  shape->blocks = p.sms * per_sm;
   shape->heads = P::NH;
   shape->split = p.max_len > kWarps * P::TK;
-  kv_attend_kernel<P><<<p.sms * per_sm, kThreads, smem, s>>>(p);
+  kv_attend_kernel<P><<<shape->blocks, kThreads, smem, s>>>(p);
   return cudaGetLastError();
 }
 

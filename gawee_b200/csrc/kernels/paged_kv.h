@@ -23,6 +23,7 @@ GAWEE_HD int kv_part_vecs(int heads, int head_dim) { return kv_part_head(heads) 
 inline int64_t kv_parts_floats(int sms, int group, int head_dim) {
   return (int64_t)2 * sms * kKvMaxBlocksPerSm * 4 * kv_part_vecs(group > 8 ? kKvHeadsMost : 8, head_dim);
 }
+inline int64_t kv_blocks(int sms) { return (int64_t)sms * kKvMaxBlocksPerSm; }
 inline int64_t kv_segments(int64_t batch, int kv_heads, int group) { return batch * kv_heads * ((group + 3) / 4); }
 // SMs that a graph's workspace is planned for; a GPU with more uses this many.
 constexpr int kKvPlanSms = 160;
@@ -72,6 +73,8 @@ struct KvAttendParams {
   float* stats;          // [batch][heads][2]: maximum and sum, with weights_out
   float* parts;          // states of parts of segments: two a block
   int2* info;            // of each segment: its first block, and the number of its blocks
+  int2* splits;          // of each block: the segment that begins in its run and goes on behind it, and
+                         // the number of its blocks (0: none)
   int device, sms;
   int page_shift;        // log2 of the page size, -1 where it is no power of two
   int* status;
@@ -79,6 +82,7 @@ struct KvAttendParams {
 cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s);
 // The same for pages of one type (paged_attend_*.cu), without the join.
 struct KvAttendShape {
+  int blocks;  // of the grid
   int heads;   // of a part: the heads that a block computes together
   bool split;  // a segment may have several tiles, and so several blocks
 };
