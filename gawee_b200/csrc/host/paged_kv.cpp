@@ -18,6 +18,8 @@ struct gawee_kv {
   gawee_kv_desc desc{};
   gawee::kern::PageGeom geom{};
   int device = -1;
+  int sms = 0;
+  void* memory = nullptr;      // one allocation, of which the rest are parts
   int* status = nullptr;       // first error a kernel reported (kern::Status)
   int32_t* plan = nullptr;     // [max_batch][2]: evict's lengths before and after
   float* stats = nullptr;      // [max_batch][heads][2], with desc.weights
@@ -25,16 +27,7 @@ struct gawee_kv {
   float* parts = nullptr;      // attend's partial states
   int2* info = nullptr;        // attend's segments and the blocks that share them
   int2* splits = nullptr;      // .. and its blocks and the segments that they leave unfinished
-  int sms = 0;
-  ~gawee_kv() {
-    cudaFree(status);
-    cudaFree(plan);
-    cudaFree(stats);
-    cudaFree(scores);
-    cudaFree(parts);
-    cudaFree(info);
-    cudaFree(splits);
-  }
+  ~gawee_kv() { cudaFree(memory); }
 };
 
 namespace {
@@ -161,21 +154,35 @@ gawee_status gawee_kv_create(const gawee_kv_desc* desc, int device, gawee_kv** o
     if (device < 0 || device >= n) return bad("invalid device index");
     DeviceScope scope(device);
     e = scope.err;
-    const size_t rows = (size_t)d.max_batch * d.heads;
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->status, sizeof(int));
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->plan, sizeof(int32_t) * 2 * d.max_batch);
-    if (e == cudaSuccess && d.weights) e = cudaMalloc((void**)&kv->stats, sizeof(float) * 2 * rows);
-    if (e == cudaSuccess && d.weights)
-      e = cudaMalloc((void**)&kv->scores, sizeof(float) * rows * d.max_pages * d.page_size);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess)
-      e = cudaMalloc((void**)&kv->parts,
-                     sizeof(float) * gawee::kern::kv_parts_floats(kv->sms, d.heads / d.kv_heads, d.head_dim));
-    if (e == cudaSuccess)
-      e = cudaMalloc((void**)&kv->info,
-                     sizeof(int2) * gawee::kern::kv_segments(d.max_batch, d.kv_heads, d.heads / d.kv_heads));
-    if (e == cudaSuccess) e = cudaMalloc((void**)&kv->splits, sizeof(int2) * gawee::kern::kv_blocks(kv->sms));
-    if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));
+    const int group = d.heads / d.kv_heads;
+    const size_t rows = (size_t)d.max_batch * d.heads;
+    size_t bytes = 0;
+    auto place = [&](size_t n) {
+      const size_t at = bytes;
+      bytes += (n + 255) / 256 * 256;
+      return at;
+    };
+    const size_t status = place(sizeof(int)), plan = place(sizeof(int32_t) * 2 * d.max_batch);
+    const size_t parts = place(sizeof(float) * gawee::kern::kv_parts_floats(kv->sms, group, d.head_dim));
+    const size_t info = place(sizeof(int2) * gawee::kern::kv_segments(d.max_batch, d.kv_heads, group));
+    const size_t splits = place(sizeof(int2) * gawee::kern::kv_blocks(kv->sms));
+    const size_t stats = place(d.weights ? sizeof(float) * 2 * rows : 0);
+    const size_t scores = place(d.weights ? sizeof(float) * rows * d.max_pages * d.page_size : 0);
+    if (e == cudaSuccess) e = cudaMalloc(&kv->memory, bytes);
+    if (e == cudaSuccess) {
+      char* m = static_cast<char*>(kv->memory);
+      kv->status = reinterpret_cast<int*>(m + status);
+      kv->plan = reinterpret_cast<int32_t*>(m + plan);
+      kv->parts = reinterpret_cast<float*>(m + parts);
+      kv->info = reinterpret_cast<int2*>(m + info);
+      kv->splits = reinterpret_cast<int2*>(m + splits);
+      if (d.weights) {
+        kv->stats = reinterpret_cast<float*>(m + stats);
+        kv->scores = reinterpret_cast<float*>(m + scores);
+      }
+      e = cudaMemset(kv->status, 0, sizeof(int));
+    }
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
       cudaGetLastError();

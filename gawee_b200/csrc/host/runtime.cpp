@@ -1365,6 +1365,10 @@ int gawee_num_launches(const gawee_ctx* ctx) {
   for (int o : ctx->rt.plan->main) {
     const auto& op = ctx->rt.plan->ops[o];
     n += 1 + (o < (int)ctx->rt.ksplit.size() && ctx->rt.ksplit[o] > 1 ? 1 : 0);
+    if (op.kind == gawee::OpKind::PAGED_ATTN) {  // reads: q, k, v, the pages, the table, ..
+      const auto &pages = op.reads[3].shape, &table = op.reads[5].shape;
+      n += gawee::kern::kv_attend_launches_f32((int)pages[3], table[1] * pages[2]) - 1;
+    }
     // the skip-flag pass, unless the mask is fixed and its flags are filled
     if (op.kind == gawee::OpKind::ATTN && op.attn.has_mask &&
         !(o < (int)ctx->rt.attn_skip_static.size() && ctx->rt.attn_skip_static[o] == 2))

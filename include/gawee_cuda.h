@@ -295,7 +295,7 @@ typedef struct {
 
 /* Write the rows of new tokens (a prompt, or one token per sequence) into the
  * pages.  Tokens with a negative sequence or position are left out.  Two
- * tokens of one call that name the same row leave one of the two there. */
+ * tokens of one call that name the same row leave a mixture of the two there. */
 gawee_status gawee_kv_append(gawee_kv* kv, const gawee_kv_append_args* args, void* stream);
 
 typedef struct {
