@@ -799,3 +799,74 @@ def test_decode_graph_of_the_15m_shapes_runs_with_the_library_calls_on_its_pages
     finally:
         a.close()
         b.close()
+
+
+# --- larger batches and what the division of the work does with them ------------------
+
+@pytest.mark.parametrize("types", TYPES[:3], ids=lambda t: f"{t[0]}-{t[1]}")
+def test_attend_many_sequences(types):
+    """More sequences than a block has threads, of all lengths, with rows of none between them."""
+    rng = np.random.default_rng(60)
+    lens = [int(x) for x in rng.choice([-1, 0, 1, 2, 3, 15, 16, 17, 40, 64, 65, 130], 700)]
+    lens[0] = lens[1] = lens[-1] = -1
+    c = Cache(rng, lens, 2, 32, 16, types[0])
+    _run(c, 6, types[1], with_weights=True, new=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attend_one_long_sequence_among_short_ones(dtype):
+    c = Cache(np.random.default_rng(61), [1, 3, 9000, 2, -1, 0, 5, 130], 2, 64, 16, dtype)
+    _run(c, 8, dtype, new=True, with_weights=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["all", "front", "back", "all_but_one"])
+def test_attend_masks_that_empty_whole_parts(dtype, kind):
+    """A mask that leaves some or all of the blocks that share a sequence without a row."""
+    c = Cache(np.random.default_rng(62), [6000, 50], 1, 64, 32, dtype)
+    mask = np.zeros((2, c.cols * c.page), np.float32)
+    mask[0, {"all": slice(None), "front": slice(0, 5900), "back": slice(70, None), "all_but_one": slice(None)}[kind]] = -np.inf
+    if kind == "all_but_one":
+        mask[0, 4321] = 0
+    _run(c, 4, dtype, mask=torch.from_numpy(mask).cuda(), with_weights=True)
+
+
+@pytest.mark.parametrize("in_place", [False, True], ids=["copied", "in_place"])
+@pytest.mark.parametrize("kind", ["random", "ties", "equal", "odd", "rising"])
+def test_evict_by_several_blocks_a_head(kind, in_place):
+    _evict([9000, 4097, 5, 8999], 2, 8, 64, "f32", 4000, 700, kind, in_place, alias=in_place)
+    _evict([9000, 4500], 1, 8, 64, "bf16", 300, 300, kind, in_place)
+    _evict([5000], 1, 8, 7, "f16", 4999, 0, kind, in_place, alias=True)
+
+
+def test_evict_many_long_sequences():
+    _evict([4200 + 7 * i for i in range(60)], 1, 8, 64, "bf16", 1000, 100, "ties", True, alias=True)
+
+
+def test_evict_many_short_sequences():
+    _evict([int(x) for x in np.random.default_rng(63).integers(-1, 90, 300)], 2, 8, 16, "f32", 30, 7, "ties", False)
+
+
+def test_append_many_tokens_of_many_sequences():
+    rng = np.random.default_rng(64)
+    c = Cache(rng, [0] * 90, 2, 16, 16, "bf16", spare_rows=70)
+    new = [(b, p) for b in range(90) for p in range(int(rng.integers(0, 70)))]
+    k, v = (_normal(rng, (len(new), 2, 16), "f32").cuda() for _ in range(2))
+    seq, pos = (torch.tensor([x[i] for x in new], dtype=torch.int32, device="cuda") for i in (0, 1))
+    h = c.handle(2)
+    h.append(c.k, c.v, k, v, c.table, pos, sequences=seq)
+    h.synchronize()
+    at = 0
+    for b in range(90):
+        n = sum(1 for x in new if x[0] == b)
+        for pages, x in ((c.k, k), (c.v, v)):
+            assert torch.equal(c.get(pages, b, n), x[at:at + n].transpose(0, 1).to(torch.bfloat16).cpu())
+        at += n
+
+
+def test_calls_leave_the_current_device_and_no_error_behind():
+    c = Cache(np.random.default_rng(65), [20], 1, 64, 16, "f32")
+    before = torch.cuda.current_device()
+    _run(c, 2, "f32")
+    assert torch.cuda.current_device() == before
+    torch.cuda.synchronize()
