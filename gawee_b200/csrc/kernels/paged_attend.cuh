@@ -1026,8 +1026,14 @@ cudaError_t attend_mma(const KvAttendParams& p, KvAttendShape* shape, cudaStream
 }
 template <class T>
 cudaError_t attend_16bit(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
-  const int group = p.heads / p.geom.kv_heads;
-  if (p.dt == TypeCode<T>::value && group > 1) return group <= 8 ? attend_mma<T, 8>(p, shape, s) : attend_mma<T, 16>(p, shape, s);
+  // Tensor cores need one type, and pay from 16 to 128 elements a row whatever the
+  // group (64 sequences of up to 1024 rows, 8 heads: 31.5 -> 21.2 us at 32
+  // elements, 36.4 -> 33.9 at 128); rows of 8 are mostly padding (18.0 -> 20.7) and longer ones leave an SM
+  // one block (192: 82 -> 118), which only the arithmetic of three heads and more
+  // outweighs (256 elements, 4 heads a key/value head, 74,862 rows: 132 -> 80).
+  const int D = p.geom.head_dim, group = p.heads / p.geom.kv_heads;
+  if (p.dt == TypeCode<T>::value && ((D >= 16 && D <= 128) || group > 2))
+    return group <= 8 ? attend_mma<T, 8>(p, shape, s) : attend_mma<T, 16>(p, shape, s);
   return attend_lanes<T>(p, shape, s);
 }
 
