@@ -53,20 +53,27 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendParam
   if (t >= p.tokens) return;
   const int64_t seq = p.sequences ? (int64_t)p.sequences[t] : t;
   const int64_t pos = p.positions[t];
-  if (seq < 0 || pos < 0) return;
   const int lane = threadIdx.x % lanes, head_vecs = p.geom.head_dim / kPer, vecs = p.geom.kv_heads * head_vecs;
+  const A *k = static_cast<const A*>(p.k) + t * p.k_stride, *v = static_cast<const A*>(p.v) + t * p.v_stride;
+  // the first vectors are on the way while the page is looked up
+  float x[kPer], y[kPer];
+  if (lane < vecs) {
+    load_n<A, kPer, ALIGNED>(k + lane * kPer, x);
+    load_n<A, kPer, ALIGNED>(v + lane * kPer, y);
+  }
+  if (seq < 0 || pos < 0) return;
   const int64_t page = seq < p.batch ? page_of(p.table + seq * p.table_stride, p.table_cols, pos, p.geom) : -1;
   if (page < 0) {
     if (lane == 0) set_status(p.status, seq < p.batch ? ST_KV_PAGE : ST_KV_SEQUENCE);
     return;
   }
   const int slot = (int)(pos % p.geom.page_size);
-  const A *k = static_cast<const A*>(p.k) + t * p.k_stride, *v = static_cast<const A*>(p.v) + t * p.v_stride;
   for (int i = lane; i < vecs; i += lanes) {
     const int64_t o = row_offset(page, i / head_vecs, slot, p.geom) + i % head_vecs * kPer;
-    float x[kPer], y[kPer];
-    load_n<A, kPer, ALIGNED>(k + i * kPer, x);
-    load_n<A, kPer, ALIGNED>(v + i * kPer, y);
+    if (i != lane) {
+      load_n<A, kPer, ALIGNED>(k + i * kPer, x);
+      load_n<A, kPer, ALIGNED>(v + i * kPer, y);
+    }
     uint4 a, b;
     T *ka = reinterpret_cast<T*>(&a), *va = reinterpret_cast<T*>(&b);
 #pragma unroll
