@@ -4,8 +4,8 @@
 what each call computes, what it leaves alone and which calls may overlap.
 The caller owns every array; the handle holds the shapes and the scratch
 memory.  Arrays are device tensors of the handle's device, of any library
-whose tensors have `data_ptr()`, `shape`, `stride()`, `dtype` and
-`get_device()` as PyTorch's do.
+whose tensors have `data_ptr()`, `shape`, `stride()`, `is_contiguous()`,
+`dtype` and `get_device()` as PyTorch's do.
 
     pages:    k_pages, v_pages [num_pages, kv_heads, page_size, head_dim]
     table:    block_table int32 [batch, columns], a sequence's pages in order
@@ -87,6 +87,7 @@ class PagedKV:
         self.heads, self.kv_heads, self.head_dim, self.page_size = heads, kv_heads, head_dim, page_size
         self._page_shape = (num_pages, kv_heads, page_size, head_dim)
         self._page_stride = page_stride or kv_heads * page_size * head_dim
+        self._dense_pages = self._page_stride == kv_heads * page_size * head_dim
         self._page_strides = (self._page_stride, page_size * head_dim, head_dim, 1)
 
     def close(self):
@@ -121,6 +122,8 @@ class PagedKV:
     def _pages(self, t, name: str) -> int:
         if t.shape != self._page_shape:
             raise _invalid(f"{name} has shape {tuple(t.shape)}, expected {self._page_shape}")
+        if self._dense_pages and t.is_contiguous():
+            return self._on_device(t, name, self._dt)
         s = t.stride()
         n, kvh, page, dim = self._page_shape
         if s != self._page_strides and (s[3] != 1 or (page > 1 and s[2] != dim) or (kvh > 1 and s[1] != page * dim)
@@ -132,19 +135,24 @@ class PagedKV:
         """(address, stride between rows) of [n, heads, head_dim] with dense rows."""
         if t.shape != (n, heads, self.head_dim):
             raise _invalid(f"{name} has shape {tuple(t.shape)}, expected {(n, heads, self.head_dim)}")
+        if t.is_contiguous():
+            return self._on_device(t, name, code), heads * self.head_dim
         s = t.stride()
         if s[2] != 1 or (heads > 1 and s[1] != self.head_dim):
             raise _invalid(f"{name} has strides {tuple(s)}: each row [heads, head_dim] is dense")
         return self._on_device(t, name, code), s[0]
 
     def _ints(self, t, name: str, n: int) -> int:
-        if t.shape != (n,) or (n > 1 and t.stride()[0] != 1):
+        if t.shape != (n,) or not t.is_contiguous():
             raise _invalid(f"{name} must be a dense array of {n} int32 values, got shape {tuple(t.shape)}")
         return self._on_device(t, name, 4)
 
     def _table(self, t, name: str):
         """(address, stride, rows, columns)"""
-        shape, s = t.shape, t.stride()
+        shape = t.shape
+        if len(shape) == 2 and t.is_contiguous():
+            return self._on_device(t, name, 4), shape[1], shape[0], shape[1]
+        s = t.stride()
         if len(shape) != 2 or (shape[1] > 1 and s[1] != 1):
             raise _invalid(f"{name} must be int32 [batch, columns] with dense rows")
         return self._on_device(t, name, 4), s[0], shape[0], shape[1]
