@@ -597,6 +597,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   __shared__ long long s_warp[kWarps], s_base;
   __shared__ int s_b0;
   __shared__ float s_ml[kWarps][NH][2];  // the warps' maxima and sums
+  __shared__ long long s_new[kWarps][NS];  // of a stage with a sequence's last row: where that is still to be stored, or -1
   asm volatile("griddepcontrol.launch_dependents;");  // the join may take its place early: it waits for this grid's end
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (tid == 0) p.splits[blockIdx.x] = make_int2(0, 0);
@@ -628,8 +629,11 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     total = sum * per_tile;
     blocks = min((long long)gridDim.x, total);  // every one of them has a unit
     if (blockIdx.x >= blocks) return;
-    u0 = total * blockIdx.x / blocks;
-    u1 = total * (blockIdx.x + 1) / blocks;
+    // floor(total * i / blocks), by one long division
+    const long long each = total / blocks;
+    const unsigned rest = (unsigned)(total - each * blocks), n = (unsigned)blocks, i = blockIdx.x;
+    u0 = each * i + rest * i / n;
+    u1 = each * (i + 1) + rest * (i + 1) / n;
     before = (before + scan - mine) * per_tile;
     if (u0 >= before && u0 < before + mine * per_tile) {  // this thread's slice holds the first unit
       int b = b0;
@@ -668,7 +672,9 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   use.tiles = tiles_of<TILE>(use.len);
   {
     const long long in = u0 - s_base;  // units into the sequence: (kvh, chunk, unit)
-    const int units = use.tiles + kStart, seg = (int)(in / units), unit = (int)(in % units);
+    const int units = use.tiles + kStart;
+    const int seg = in >> 32 ? (int)(in / units) : (int)((unsigned)in / (unsigned)units);
+    const int unit = (int)(in - (long long)seg * units);
     use.tile = max(unit - kStart, 0);
     use.chunk = seg % chunks;
     use.kvh = seg / chunks;
@@ -806,9 +812,14 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         }
         return;
       }
-      // the new token's row is written below, unless the mask takes it out
+      // The new token's row comes from the call's arguments.  In the pages' type
+      // it is copied like the others and stored when its tile is used; another
+      // type is rounded and stored below.  A row that the mask takes out stays zeros.
       const int new_row = fresh_row ? __ffs(fresh_row) - 1 : 0;
-      const bool put_new = fresh_row && __shfl_sync(0xffffffffu, f_add, new_row) != -INFINITY;
+      const bool live_new = fresh_row && __shfl_sync(0xffffffffu, f_add, new_row) != -INFINITY;
+      const bool copy_new = live_new && p.k_as_stored, put_new = live_new && !copy_new;
+      const int64_t k_new = c.b * p.k_stride + c.kvh * D, v_new = c.b * p.v_stride + c.kvh * D;
+      if (p.k_as_stored && first + TK >= c.len && lane == 0) s_new[warp][stage] = copy_new ? fresh_off : -1;
       int row = row_0, col = col_0;
       for (int v = 0; v < TK * vecs; v += 32) {
         const long long o = __shfl_sync(0xffffffffu, off, row & 31);
@@ -816,8 +827,13 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
           const bool ok = o >= 0;
           const long long at = ok ? o + col * 16 : 0;
           const int s = row * rb + P::chunk_at(row, col, D) * 16;
-          copy16(smem_u32(ks + s), static_cast<const char*>(p.k_pages) + at, ok);
-          copy16(smem_u32(vs + s), static_cast<const char*>(p.v_pages) + at, ok);
+          if (copy_new && row == new_row) {
+            copy16(smem_u32(ks + s), reinterpret_cast<const char*>(static_cast<const T*>(p.k) + k_new) + col * 16);
+            copy16(smem_u32(vs + s), reinterpret_cast<const char*>(static_cast<const T*>(p.v) + v_new) + col * 16);
+          } else {
+            copy16(smem_u32(ks + s), static_cast<const char*>(p.k_pages) + at, ok);
+            copy16(smem_u32(vs + s), static_cast<const char*>(p.v_pages) + at, ok);
+          }
         }
         row += row_step;
         col += col_step;
@@ -826,18 +842,16 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
           ++row;
         }
       }
-      if (fresh_row) {
-        // the new token's row comes from the call's arguments, rounded as it is
-        // stored; the block of the first chunk of heads stores it
+      if (fresh_row && !copy_new) {
         for (int d = lane; d < D; d += 32) {
-          const T k = from_f<T>(load_act(p.k, p.dt, c.b * p.k_stride + c.kvh * D + d));
-          const T v = from_f<T>(load_act(p.v, p.dt, c.b * p.v_stride + c.kvh * D + d));
+          const T k = from_f<T>(load_act(p.k, p.dt, k_new + d));
+          const T v = from_f<T>(load_act(p.v, p.dt, v_new + d));
           if (put_new) {
             const int s = new_row * rb + P::chunk_at(new_row, d * (int)sizeof(T) / 16, D) * 16 + d * (int)sizeof(T) % 16;
             *reinterpret_cast<T*>(ks + s) = k;
             *reinterpret_cast<T*>(vs + s) = v;
           }
-          if (c.chunk == 0) {
+          if (c.chunk == 0) {  // the block of the first chunk of heads stores it
             reinterpret_cast<T*>(static_cast<char*>(p.k_pages) + fresh_off)[d] = k;
             reinterpret_cast<T*>(static_cast<char*>(p.v_pages) + fresh_off)[d] = v;
           }
@@ -893,6 +907,17 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         copy_commit();
         load_stage = load_stage + 1 == NS ? 0 : load_stage + 1;
         stage_at = stage * stage_bytes;
+        if (p.k_as_stored && use.chunk == 0 && first < use.len && first + TK >= use.len) {  // the tile of the last row
+          const int row = use.len - 1 - first;
+          const long long to = s_new[warp][stage];
+          if (to >= 0)
+            for (int v = lane; v < 2 * vecs; v += 32) {
+              const int col = v < vecs ? v : v - vecs;
+              const char* from = ring + stage_at + (v < vecs ? 0 : TK * rb) + row * rb + P::chunk_at(row, col, D) * 16;
+              *reinterpret_cast<uint4*>(static_cast<char*>(v < vecs ? p.k_pages : p.v_pages) + to + col * 16) =
+                  *reinterpret_cast<const uint4*>(from);
+            }
+        }
         if (first < use.len)
           state.tile(ring + stage_at, ring + stage_at + TK * rb, adds + stage * TK, scratch, queries, scores,
                      use.len - first, group, nh);
@@ -939,7 +964,8 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
       if (tid == 0 && begins) {
         // for the join: the segment's first block and the number of its blocks; the
         // block that holds unit u is the largest i with floor(total * i / blocks) <= u
-        const int last = (int)(((seg_begin + use.tiles + kStart) * blocks - 1) / total);
+        const long long u = (seg_begin + use.tiles + kStart) * blocks - 1;
+        const int last = u >> 32 ? (int)(u / total) : (int)((unsigned)u / (unsigned)total);  // u >= total - 1: both fit
         const int segment = (use.b * kv + use.kvh) * chunks + use.chunk, n = last - (int)blockIdx.x + 1;
         p.info[segment] = make_int2(blockIdx.x, n);
         if (n > 1) p.splits[blockIdx.x] = make_int2(segment, n);

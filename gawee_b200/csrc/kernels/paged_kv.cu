@@ -133,13 +133,15 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
   extern __shared__ float4 s_join[];
   const int kv = p.geom.kv_heads, D = p.geom.head_dim, group = p.heads / kv, chunks = (group + heads - 1) / heads;
   const int tid = threadIdx.x, warp = tid / 32;
+  const bool none = (int)blockIdx.x < joins && by_segment &&  // lengths were there before the attention began
+                    p.lengths[blockIdx.x / min(heads, group) / chunks / kv] < 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the attention has ended and its results are visible
+  if (none) return;
   if ((int)blockIdx.x < joins) {
     const int most = min(heads, group), index = blockIdx.x / most, h = blockIdx.x % most;
     int segment = index;
     int2 info;  // the segment's first block and the number of its blocks
     if (by_segment) {
-      if (p.lengths[segment / chunks / kv] < 0) return;
       info = p.info[segment];
     } else {
       const int2 split = p.splits[index];
@@ -582,8 +584,13 @@ cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t s) {
   });
 }
 
-cudaError_t launch_kv_attend(const KvAttendParams& p, cudaStream_t s) {
-  if (p.batch == 0) return cudaSuccess;
+cudaError_t launch_kv_attend(const KvAttendParams& given, cudaStream_t s) {
+  if (given.batch == 0) return cudaSuccess;
+  KvAttendParams p = given;
+  auto rows_aligned = [&](const void* at, int64_t stride) {
+    return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (p.batch == 1 || stride * elem_bytes(p.dt) % 16 == 0);
+  };
+  p.k_as_stored = p.k && p.dt == p.page_dt && rows_aligned(p.k, p.k_stride) && rows_aligned(p.v, p.v_stride);
   KvAttendShape shape{};
   cudaError_t e = p.page_dt == DT_F32   ? launch_kv_attend_f32(p, &shape, s)
                   : p.page_dt == DT_F16 ? launch_kv_attend_f16(p, &shape, s)

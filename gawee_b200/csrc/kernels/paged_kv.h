@@ -69,6 +69,7 @@ struct KvAttendParams {
   int64_t max_len;  // a longer length is an error
   const void *k, *v;  // the new token's row, stored first (nullptr: none)
   int64_t k_stride, v_stride;
+  bool k_as_stored;      // k and v have the pages' type and 16-byte aligned rows (set by launch_kv_attend)
   const float* mask;
   int64_t mask_stride;
   const float* weights;  // accumulators before (nullptr with weights_out set: zeros) ..

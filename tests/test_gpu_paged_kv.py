@@ -870,3 +870,33 @@ def test_calls_leave_the_current_device_and_no_error_behind():
     _run(c, 2, "f32")
     assert torch.cuda.current_device() == before
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("types", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")], ids=lambda t: f"{t[0]}-{t[1]}")
+@pytest.mark.parametrize("offset", [0, 1, 4])
+def test_new_rows_of_any_alignment_masked_and_on_bad_pages(types, offset):
+    """New rows that start on a 16-byte boundary or do not; one that the mask
+    takes out (stored all the same), one whose page is bad (not stored)."""
+    from gawee_b200.runtime import GaweeError
+    rng = np.random.default_rng(70)
+    c = Cache(rng, [17, 64, 65, 1, 130], 2, 64, 16, types[0])
+    flat = [_normal(rng, (offset + 5 * 136,), types[1]).cuda() for _ in range(2)]
+    k, v = (f.as_strided((5, 2, 64), (136, 64, 1), offset) for f in flat)
+    q = _normal(rng, (5, 8, 64), types[1]).cuda()
+    mask = torch.zeros((5, c.cols * 16), device="cuda")
+    mask[1, 63] = -float("inf")
+    c.table[4, 8] = c.num_pages + 5
+    before = [c.k.clone(), c.v.clone()]
+    h = c.handle(8)
+    out = h.attend(c.k, c.v, q, c.table, c.lengths(), torch.empty_like(q), k=k, v=v, mask=mask)
+    with pytest.raises(GaweeError, match="block table"):
+        h.synchronize()
+    for i in range(4):
+        n = c.lens[i]
+        for which, x in ((0, k), (1, v)):
+            c.rows[i][which][:, n - 1] = x[i].cpu().to(T[types[0]])
+            before[which][int(c.table_np[i, (n - 1) // 16]), :, (n - 1) % 16] = x[i].to(T[types[0]])
+    for got, want in zip((c.k, c.v), before):
+        assert torch.equal(torch.nan_to_num(got.float(), nan=9.0), torch.nan_to_num(want.float(), nan=9.0))
+    c.lens[4] = 128  # its other rows are attended as they are
+    _check_attend(c, q, out, types[1], 0.125, mask)
