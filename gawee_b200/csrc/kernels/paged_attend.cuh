@@ -11,7 +11,7 @@
 //     evenly over a fixed grid of resident blocks: a block takes a contiguous
 //     run of tiles, whatever the lengths are, and goes through several short
 //     segments or through a part of a long one.  A segment's begin and end cost
-//     about as much as a tile, and count as one.  The lengths are read on the
+//     as much as a tile or two, and count like them.  The lengths are read on the
 //     device, so the balance needs nothing from the host.
 //   * A warp takes its own rows of each tile, through a ring of shared-memory
 //     stages of its own that cp.async fills: warps wait for no other until
@@ -570,11 +570,14 @@ template <int TILE>
 __device__ __forceinline__ int tiles_of(int len) {  // an empty sequence takes one, for its zeros
   return len < 0 ? 0 : len == 0 ? 1 : (len + TILE - 1) / TILE;
 }
-// Units of work of a segment: tile i is done by the block that has unit i + kStart.
-constexpr int kStart = 1;
+// Units of work of a segment: `start` for its begin and end, then one a tile;
+// tile i is done by the block that has unit i + start.  With four tiles a block
+// and more the begin counts as two (9/3 x 64 heads, 64 sequences of up to 2048
+// rows, fp32: 30.4 us against 32.0); with fewer as one, or blocks that hold
+// nothing else would stand idle (one of 16,385 rows: 14.4 us against 16.1).
 template <int TILE>
-__device__ __forceinline__ int units_of(int len) {
-  return len < 0 ? 0 : tiles_of<TILE>(len) + kStart;
+__device__ __forceinline__ int units_of(int len, int start) {
+  return len < 0 ? 0 : tiles_of<TILE>(len) + start;
 }
 
 // Shared memory in bytes: the warps' stages, their mask values and scratch, and the queries.  At
@@ -606,11 +609,13 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
 
   // The block's run of tiles: prefix sums of the sequences' tiles, each thread a slice of the batch.
   long long u0, u1, total, blocks;  // its units
+  int start;
   {
     const int slice = (p.batch + kThreads - 1) / kThreads, b0 = min(tid * slice, p.batch), b1 = min(b0 + slice, p.batch);
     long long mine = 0;
     for (int b = b0; b < b1; ++b) {
-      mine += units_of<TILE>(length_of(p, b));
+      const int len = length_of(p, b);
+      if (len >= 0) mine += ((long long)tiles_of<TILE>(len) << 17) + 1;  // tiles, and sequences in the low bits
       if (blockIdx.x == 0 && p.lengths[b] > p.max_len) set_status(p.status, ST_KV_LENGTH);  // length_of takes it as 0
     }
     long long scan = mine;
@@ -626,7 +631,9 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
       if (w == warp) before = sum;
       sum += s_warp[w];
     }
-    total = sum * per_tile;
+    start = (sum >> 17) * per_tile >= 4ll * gridDim.x ? 2 : 1;
+    auto units = [&](long long x) { return ((x >> 17) + (x & 0x1ffff) * start) * per_tile; };
+    total = units(sum);
     blocks = min((long long)gridDim.x, total);  // every one of them has a unit
     if (blockIdx.x >= blocks) return;
     // floor(total * i / blocks), by one long division
@@ -634,11 +641,11 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     const unsigned rest = (unsigned)(total - each * blocks), n = (unsigned)blocks, i = blockIdx.x;
     u0 = each * i + rest * i / n;
     u1 = each * (i + 1) + rest * (i + 1) / n;
-    before = (before + scan - mine) * per_tile;
-    if (u0 >= before && u0 < before + mine * per_tile) {  // this thread's slice holds the first unit
+    before = units(before + scan - mine);
+    if (u0 >= before && u0 < before + units(mine)) {  // this thread's slice holds the first unit
       int b = b0;
       for (;; ++b) {
-        const long long n = (long long)units_of<TILE>(length_of(p, b)) * per_tile;
+        const long long n = (long long)units_of<TILE>(length_of(p, b), start) * per_tile;
         if (u0 < before + n) break;
         before += n;
       }
@@ -672,16 +679,16 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
   use.tiles = tiles_of<TILE>(use.len);
   {
     const long long in = u0 - s_base;  // units into the sequence: (kvh, chunk, unit)
-    const int units = use.tiles + kStart;
+    const int units = use.tiles + start;
     const int seg = in >> 32 ? (int)(in / units) : (int)((unsigned)in / (unsigned)units);
     const int unit = (int)(in - (long long)seg * units);
-    use.tile = max(unit - kStart, 0);
+    use.tile = max(unit - start, 0);
     use.chunk = seg % chunks;
     use.kvh = seg / chunks;
   }
   long long seg_begin = 0;  // the segment's first unit
   {
-    const int units = use.tiles + kStart;
+    const int units = use.tiles + start;
     seg_begin = s_base + ((long long)use.kvh * chunks + use.chunk) * units;
   }
   // tiles of the run: a walk over its segments
@@ -690,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
     Cursor c = use;
     long long at = seg_begin;
     for (;;) {
-      const long long end = at + kStart + c.tiles, upto = min(end, u1) - at - kStart;  // tiles of the segment before u1
+      const long long end = at + start + c.tiles, upto = min(end, u1) - at - start;  // tiles of the segment before u1
       if (upto > c.tile) count += (int)upto - c.tile;
       at = end;
       if (at >= u1) break;
@@ -964,7 +971,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
       if (tid == 0 && begins) {
         // for the join: the segment's first block and the number of its blocks; the
         // block that holds unit u is the largest i with floor(total * i / blocks) <= u
-        const long long u = (seg_begin + use.tiles + kStart) * blocks - 1;
+        const long long u = (seg_begin + use.tiles + start) * blocks - 1;
         const int last = u >> 32 ? (int)(u / total) : (int)((unsigned)u / (unsigned)total);  // u >= total - 1: both fit
         const int segment = (use.b * kv + use.kvh) * chunks + use.chunk, n = last - (int)blockIdx.x + 1;
         p.info[segment] = make_int2(blockIdx.x, n);
@@ -973,7 +980,7 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
       if (j < count) put_q();
       __syncthreads();  // the stages are free again, and the next queries there
       if (padded) clear(ring + stage_at, stage_bytes);
-      seg_begin += use.tiles + kStart;
+      seg_begin += use.tiles + start;
     }
     if (j < count) advance(use);
   }
