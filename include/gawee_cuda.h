@@ -339,6 +339,7 @@ typedef struct {
  *   - A mask value of -inf takes the row out, whatever its K and V hold.  Other
  *     values are added as they are: a mask of the lowest finite value is one.
  *     A sequence of length 0, or whose rows are all taken out, gives zeros.
+ *     A mask value of +inf or NaN gives NaN.
  *   - A negative length marks a batch row without a sequence: its rows of out,
  *     weights_out and the pages are left as they were.
  *   - The same call gives the same bits: partial sums are joined in a fixed
