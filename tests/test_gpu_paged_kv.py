@@ -900,3 +900,69 @@ def test_new_rows_of_any_alignment_masked_and_on_bad_pages(types, offset):
         assert torch.equal(torch.nan_to_num(got.float(), nan=9.0), torch.nan_to_num(want.float(), nan=9.0))
     c.lens[4] = 128  # its other rows are attended as they are
     _check_attend(c, q, out, types[1], 0.125, mask)
+
+
+def test_captured_append_step_and_eviction():
+    """append, attend with weights and evict in place in one graph, replayed on
+    new inputs: as many times as the same calls made one by one."""
+    rng = np.random.default_rng(80)
+    caches = [Cache(np.random.default_rng(81), [60, 33, 1], 2, 64, 16, "bf16", spare_rows=80) for _ in range(2)]
+    state = []
+    for c in caches:
+        n = c.cols * c.page
+        state.append(dict(h=c.handle(8, weights=True), w=torch.zeros((3, 2, n), device="cuda"), lens=c.lengths(),
+                          kept=torch.zeros((3, 2, 40), dtype=torch.int32, device="cuda"),
+                          q=torch.zeros((3, 8, 64), dtype=torch.bfloat16, device="cuda"),
+                          kv=[torch.zeros((3, 2, 64), dtype=torch.bfloat16, device="cuda") for _ in range(4)],
+                          out=torch.zeros((3, 8, 64), dtype=torch.bfloat16, device="cuda")))
+
+    def step(c, s, stream):
+        s["h"].append(c.k, c.v, s["kv"][0], s["kv"][1], c.table, s["lens"], stream=stream)  # one row more ..
+        s["lens"] += 2                                                                     # .. and the step's own
+        s["h"].attend(c.k, c.v, s["q"], c.table, s["lens"], s["out"], k=s["kv"][2], v=s["kv"][3], weights=s["w"],
+                      weights_out=s["w"], stream=stream)
+        s["h"].evict(c.k, c.v, s["w"], c.table, s["lens"], 40, 8, s["kept"], s["w"], s["lens"], stream=stream)
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(caches[0], state[0], torch.cuda.current_stream())
+    for _ in range(6):
+        new = [_normal(rng, t.shape, "bf16") for t in [state[0]["q"]] + state[0]["kv"]]
+        for s in state:
+            for t, x in zip([s["q"]] + s["kv"], new):
+                t.copy_(x)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+            step(caches[1], state[1], stream)
+        for s in state:
+            s["h"].synchronize(stream)
+        for name in ("out", "w", "lens", "kept"):
+            assert torch.equal(state[0][name], state[1][name]), name
+        for a, b in ((caches[0].k, caches[1].k), (caches[0].v, caches[1].v)):
+            assert torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float()))
+    assert state[0]["lens"].tolist() == [40, 40, 13]
+
+
+def test_two_handles_at_the_same_time():
+    """Calls that overlap, on two streams with a handle each, as many as the caller likes."""
+    cs = [Cache(np.random.default_rng(82 + i), [900, 5, 2000][::1 - 2 * i], 2, 64, 16, ("f32", "bf16")[i]) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in cs]
+    handles = [c.handle(8, weights=True) for c in cs]
+    qs = [_normal(np.random.default_rng(1), (3, 8, 64), c.dtype).cuda() for c in cs]
+    lens = [c.lengths() for c in cs]
+    ws = [torch.zeros((3, 2, c.cols * c.page), device="cuda") for c in cs]
+    outs = [[torch.empty_like(q) for _ in range(15)] for q in qs]
+    wos = [[torch.zeros_like(w) for _ in range(15)] for w in ws]
+    torch.cuda.synchronize()
+    for r in range(15):
+        for i, c in enumerate(cs):
+            handles[i].attend(c.k, c.v, qs[i], c.table, lens[i], outs[i][r], weights=ws[i], weights_out=wos[i][r],
+                              stream=streams[i])
+    for i, c in enumerate(cs):
+        handles[i].synchronize(streams[i])
+        for r in range(15):
+            assert torch.equal(outs[i][r], outs[i][0]) and torch.equal(wos[i][r], wos[i][0])
+        _check_attend(c, qs[i], outs[i][0], c.dtype, 0.125, None, ws[i], wos[i][0], ws[i])
