@@ -218,7 +218,8 @@ gawee_status gawee_kv_append(gawee_kv* kv, const gawee_kv_append_args* a, void* 
     if (a->tokens < 0 || a->tokens > INT32_MAX) return bad("tokens outside 0 .. 2^31 - 1");
     if (a->tokens == 0) return GAWEE_OK;
     if (!a->k || !a->v || !a->positions) return bad("null k, v or positions");
-    if (!aligned(a->k, size_of(a->dtype)) || !aligned(a->v, size_of(a->dtype))) return bad("k or v is not aligned to its type");
+    if (!aligned(a->k, size_of(a->dtype)) || !aligned(a->v, size_of(a->dtype)))
+      return bad("k or v is not aligned to its type");
     if (!aligned(a->positions, 4) || !aligned(a->sequences, 4)) return bad("positions or sequences is not 4-byte aligned");
     if (!a->sequences && a->tokens > a->batch) return bad("more tokens than sequences, and no `sequences`");
     const int64_t row = (int64_t)kv->geom.kv_heads * kv->geom.head_dim;

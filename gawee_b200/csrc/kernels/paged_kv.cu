@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
     }
     const int chunk = segment % chunks, kvh = segment / chunks % kv, b = segment / chunks / kv;
     const int head = chunk * heads + h;
-    if (info.y <= 1 || head >= group) return;
+    // a sequence outside the batch: the scratch of another call, which overlaps against the rule
+    if (info.y <= 1 || head >= group || b >= p.batch) return;
     const int dv = D / 4, part = kv_part_vecs(heads, D);
     int lanes = 2;  // threads of a group: one for each 16 bytes of the row
     while (lanes < dv) lanes *= 2;
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(KvEvictParams p, 
   const int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
   const int tid = threadIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the selection has ended
-  const int len = p.plan[2 * b], left = max(min(len, p.budget), 0);
+  const int len = (int)min((int64_t)p.plan[2 * b], p.max_len), left = max(min(len, p.budget), 0);
   float* wo = p.weights_out + b * p.wo_batch + kvh * p.wo_stride;
   // zeros from the new length to the old one: by all blocks, or, where the
   // weights themselves are overwritten, by the block that has read them

@@ -247,8 +247,9 @@ gawee_status gawee_matmul_f32_noalloc(const float* a, const float* b, float* c, 
  *     calling thread's current device as it was.
  *   - Calls on one handle share its scratch: they are ordered by the caller,
  *     by one stream or by events; replays of graphs that hold them too.  Calls
- *     that may run at the same time take a handle each.  (Nothing of one call stays in the
- *     scratch for the next: calls that overlapped spoil only their own results.)
+ *     that may run at the same time take a handle each.  (Nothing of one call
+ *     stays in the scratch for the next: calls that overlap against this rule
+ *     spoil their own results, and no later ones.)
  *   - A bad argument is refused with GAWEE_ERR_INVALID before anything is
  *     enqueued; the message is read with gawee_last_error(NULL, ...).
  *   - What only the device can see (a table entry that names no page, a length
@@ -259,8 +260,8 @@ typedef struct gawee_kv gawee_kv;
 
 typedef struct {
   int dtype;           /* of the pages: GAWEE_F32, GAWEE_F16 or GAWEE_BF16 */
-  int heads;           /* query heads, a multiple of kv_heads, up to 4096: query head h reads key/value head h / (heads / kv_heads) */
-  int kv_heads;
+  int heads;           /* query heads, a multiple of kv_heads, up to 4096 */
+  int kv_heads;        /* query head h reads key/value head h / (heads / kv_heads) */
   int head_dim;        /* a multiple of 8, up to 256 */
   int page_size;       /* rows of a page, up to 65536 */
   int64_t num_pages;
