@@ -351,8 +351,13 @@ struct LaneTile {
 // by mma.m16n8k16 with the query heads as rows: the multiplications cost next
 // to nothing beside the loads, where the lanes' fp32 would bound a larger
 // group.  q and K are exact operands.  P is not rounded to the 16-bit type: it
-// is split into two terms (p = hi + lo, relative error 2^-16 in bf16, 2^-21 in
-// fp16).  With up to eight heads hi takes rows 0-7 and lo rows 8-15 of the
+// is split into two terms, p = hi + lo.  In bf16 their relative error is 2^-16
+// over fp32's whole range.  fp16 ends at 2^-24, so 2^15 p is split (at most
+// 32768 of 65504) and the sums of values are scaled back at the end: relative error
+// 2^-21, and 2^-40 of the largest weight where that is more.  (Split as it is, p
+// would be lost below 2^-25: 8192 keys 17.4 below one score kept three
+// quarters of their share, 32 keys nothing.)  The sum of the weights takes p itself.
+// With up to eight heads hi takes rows 0-7 and lo rows 8-15 of the
 // same product.  D is padded to DT in shared memory; rows are swizzled by 16-byte
 // chunks so that ldmatrix reads eight rows without bank conflicts.
 // With FULL, D is DT: no padding.
@@ -369,6 +374,7 @@ struct MmaTile {
   static constexpr int kD = FULL ? DT : 0;
   static constexpr int R = NH / 8;  // head rows of a thread
   static constexpr int kMinBlocks = DT == 256 ? 1 : 2;
+  static constexpr float kUp = TypeCode<T>::value == DT_F16 ? 32768.f : 1.f;  // of the weights in the products
   static_assert(2 * TK * DT * 2 >= NH * DT * 4, "a warp's state fits into a stage");
 
   uint32_t q[DT / 16][2 * R];
@@ -429,8 +435,12 @@ struct MmaTile {
                  : "r"(at)
                  : "memory");
   }
-  // Two values as the 16-bit type, and what the rounding left.
+  // Two weights, times kUp, as the 16-bit type, and what the rounding left.
   __device__ static __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    if constexpr (kUp != 1.f) {
+      x *= kUp;
+      y *= kUp;
+    }
     T h[2] = {from_f<T>(x), from_f<T>(y)};
     T r[2] = {from_f<T>(x - to_f(h[0])), from_f<T>(y - to_f(h[1]))};
     hi = *reinterpret_cast<uint32_t*>(h);
@@ -551,8 +561,10 @@ struct MmaTile {
       for (int j = 0; j < DT / 8; ++j) {
         const int d = j * 8 + lane % 4 * 2;
         if (d < D) {
-          o[head * D + d] = R == 1 ? acc[j][0] + acc[j][2] : acc[j][2 * r];
-          o[head * D + d + 1] = R == 1 ? acc[j][1] + acc[j][3] : acc[j][2 * r + 1];
+          const float x = R == 1 ? acc[j][0] + acc[j][2] : acc[j][2 * r];
+          const float y = R == 1 ? acc[j][1] + acc[j][3] : acc[j][2 * r + 1];
+          o[head * D + d] = kUp == 1.f ? x : x * (1.f / kUp);
+          o[head * D + d + 1] = kUp == 1.f ? y : y * (1.f / kUp);
         }
       }
     }

@@ -331,7 +331,10 @@ typedef struct {
 
 /* Attention of one new token per sequence over its rows 0 .. length - 1:
  *   out[b][h] = sum_i p_i V_i,  p = softmax_i(scale * (q[b][h] . K_i) + mask[b][i]),
- * with fp32 scores, maxima and sums.  With k and v, they are first stored as
+ * with fp32 scores, maxima and sums.  Where pages and activations are of one 16-bit
+ * type, the weights may enter the products with V as two terms of that type: off by 2^-16
+ * relatively in bf16, in f16 by 2^-21 or by 2^-40 of the largest weight,
+ * whichever is more; otherwise they are fp32.  With k and v, they are first stored as
  * row length - 1 (rounded to the pages' type, and attended as stored); the
  * page of that row then belongs to this sequence alone.  With weights_out,
  * each row's weights, summed over the query heads that share its key/value

@@ -1,0 +1,65 @@
+"""Paged key/value cache on the GPU where its numbers reach their limits:
+dominant scores, values that are not finite."""
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_paged_kv import T, U, Cache, _half_step, _reference, _run
+
+pytestmark = pytest.mark.gpu
+
+
+def _sink(c, gap, values):
+    """Sequence 0 of `c` takes the given values and zero keys, but for one row: its key gives a query of
+    (1, 0, ..) the score `gap`, and its value is zero."""
+    n = c.lens[0]
+    at = n // 3
+    k, v = torch.zeros(c.kv_heads, n, c.dim), values
+    k[:, at, 0] = gap
+    v[:, at] = 0.0
+    c.rows[0] = [k.to(T[c.dtype]), v.to(T[c.dtype])]
+    c.put(0)
+
+
+# head dims and groups of every tensor-core form: 8 and 16 rows, dims that fill a form and that do not
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (16, 1, 64), (8, 2, 128), (12, 1, 128), (3, 1, 40), (8, 1, 200),
+                                          (10, 1, 256)])
+@pytest.mark.parametrize("gap", [9, 12, 15, 17, 18, 22])
+def test_attend_keeps_the_small_weights_beside_a_dominant_score(dtype, heads, kv, dim, gap):
+    """One key's score is far above the others' and its value is zero, as with
+    an attention sink: the result is what the others' small weights leave.
+
+    The scores are exact (one product each, of whole numbers).  A weight's
+    numerator is off by 8 u relatively and by 2^-16 (two bf16 terms), or by
+    2^-21 and, absolutely, 2^-40 of the largest (two fp16 terms): over n keys
+    n 2^-40 max |v| / l, with l >= 1.  Sums over n rows as tensor cores add them:
+    (n + 24) 4 u, of numerator and denominator.
+    """
+    for n in (33, 8192):
+        rng = np.random.default_rng(n + gap)
+        c = Cache(rng, [n], kv, dim, 16, dtype)
+        _sink(c, gap, torch.from_numpy(rng.uniform(100, 1000, (kv, n, dim)).astype(np.float32)))
+        q = torch.zeros(1, heads, dim, dtype=T[dtype])
+        q[:, :, 0] = 1
+        q = q.cuda()
+        h = c.handle(heads)
+        out = h.attend(c.k, c.v, q, c.table, c.lengths(), torch.empty_like(q), scale=1.0)
+        h.synchronize()
+        ref, mag, _, _ = _reference(q[0].cpu(), c.rows[0][0], c.rows[0][1], 1.0, None)
+        terms, floor = (2.0 ** -21, 2.0 ** -40) if dtype == "f16" else (2.0 ** -16, 0.0)
+        rel = 2 * ((n + 24) * 4 * U + terms)
+        tol = rel * mag + n * floor * 1000 + _half_step(dtype) * (1 + rel) * np.abs(ref)
+        if dtype == "f16":
+            tol = tol + 2.0 ** -25  # half the smallest step of fp16
+        err = np.abs(out[0].cpu().double().numpy() - ref)
+        assert (err <= tol).all(), f"{n} rows: off by {err.max():.3e} of {np.abs(ref).max():.3e}, {(err / tol).max():.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (24, 2, 128), (8, 1, 200)])
+def test_attend_large_fp16_scores(heads, kv, dim):
+    """Scores of some hundreds, of both signs, in fp16: the running maximum moves by far."""
+    c = Cache(np.random.default_rng(6), [500, 37, 1025], kv, dim, 16, "f16")
+    _run(c, heads, "f16", q_scale=60.0)
+    _run(c, heads, "f16", q_scale=60.0, scale=-0.125)
+    _run(c, heads, "f16", scale=0.0)
