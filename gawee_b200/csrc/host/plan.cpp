@@ -1882,6 +1882,7 @@ class Planner {
           p.numel() != plan_->bufs[p.buf].elems)
         unsupported("paged_attention: the pages must be function arguments f32 [pages, kv_heads, page_size, D]");
       if (!page_bufs_.insert(p.buf).second) unsupported("paged_attention: a pages argument used twice");
+      plan_->in_place_args.insert(plan_->bufs[p.buf].arg);
     }
     View table = value_view(n.ins[5]), lengths = value_view(n.ins[6]);
     const int64_t B = q.shape[0], H = q.shape[1], D = q.shape[2], KV = k.shape[1];

@@ -118,6 +118,7 @@ struct Plan {
   std::vector<View> value_view;  // per graph value
   std::vector<int> arg_buf;      // per argument
   std::vector<View> result_view; // per result (dense row-major)
+  std::set<int> in_place_args;   // arguments that the forward writes: the pages of paged_attention ops
   std::vector<int> prologue, pack, main;  // op indices per phase, in order
   size_t arena_bytes = 0, persist_bytes = 0;
   std::string summary() const;  // one line per main op: its name and execution_note

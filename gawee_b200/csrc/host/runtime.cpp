@@ -11,6 +11,7 @@
 #include <cstdlib>
 #include <cmath>
 #include <cstring>
+#include <map>
 #include <memory>
 #include <mutex>
 #include <sstream>
@@ -1280,6 +1281,24 @@ gawee_status gawee_arg_device_ptr(gawee_ctx* ctx, int i, void** ptr) {
   });
 }
 
+int gawee_arg_in_place(const gawee_ctx* ctx, int i) {
+  if (!ctx || i < 0 || i >= gawee_num_args(ctx)) return -1;
+  return ctx->rt.plan->in_place_args.count(i) ? 1 : 0;
+}
+
+gawee_status gawee_get_arg(gawee_ctx* ctx, int i, void* host, size_t bytes, void* stream) {
+  if (!ctx) return GAWEE_ERR_INVALID;
+  return guard(ctx, [&] {
+    auto& rt = ctx->rt;
+    if (!rt.plan->in_place_args.count(i))
+      throw gawee::StatusError(GAWEE_ERR_INVALID, "argument " + std::to_string(i) + " is not one that the forward writes");
+    const gawee::Buf& b = rt.plan->bufs[rt.plan->arg_buf[i]];
+    if (bytes != b.bytes() || !host)
+      throw gawee::StatusError(GAWEE_ERR_INVALID, "argument " + std::to_string(i) + " has " + std::to_string(b.bytes()) + " bytes");
+    GCHECK(cudaMemcpyAsync(host, b.ptr, bytes, cudaMemcpyDeviceToHost, stream_of(ctx, stream)));
+  });
+}
+
 gawee_status gawee_forward(gawee_ctx* ctx, void* stream) {
   if (!ctx) return GAWEE_ERR_INVALID;
   return guard(ctx, [&] { ctx->rt.forward(stream_of(ctx, stream)); });
@@ -1458,6 +1477,7 @@ gawee_status gawee_ciface_forward(gawee_ctx* ctx, void* result_desc, void* const
     if (nargs != (int)g.args.size()) throw gawee::StatusError(GAWEE_ERR_INVALID, "wrong number of memref arguments");
     if (g.results.size() != 1) throw gawee::StatusError(GAWEE_ERR_UNSUPPORTED, "the ciface entry supports one result");
     cudaStream_t s = rt.own_stream;
+    std::map<int, void*> in_place;  // the caller's memory of the arguments that the forward writes
     for (int a = 0; a < nargs; ++a) {
       const auto& t = g.values[g.args[a]].type;
       const char* d = static_cast<const char*>(arg_descs[a]);
@@ -1475,9 +1495,9 @@ gawee_status gawee_ciface_forward(gawee_ctx* ctx, void* result_desc, void* const
         expect *= t.shape[k];
       }
       const gawee::Buf& b = rt.plan->bufs[rt.plan->arg_buf[a]];
-      if (b.ptr)
-        GCHECK(cudaMemcpyAsync(b.ptr, aligned + offset * (int64_t)gawee::dtype_size(t.dtype), b.bytes(),
-                               cudaMemcpyHostToDevice, s));
+      const char* data = aligned + offset * (int64_t)gawee::dtype_size(t.dtype);
+      if (b.ptr) GCHECK(cudaMemcpyAsync(b.ptr, data, b.bytes(), cudaMemcpyHostToDevice, s));
+      if (rt.plan->in_place_args.count(a)) in_place[a] = const_cast<char*>(data);
       rt.dirty[a] = 1;
     }
     rt.forward(s);
@@ -1485,8 +1505,12 @@ gawee_status gawee_ciface_forward(gawee_ctx* ctx, void* result_desc, void* const
     size_t nb = (size_t)v.numel() * gawee::dtype_size(v.dt);
     void* host = std::malloc(nb ? nb : 1);  // owned by the caller, as in the reference ABI
     if (!host) throw gawee::StatusError(GAWEE_ERR_OOM, "malloc of the result failed");
-    GCHECK(cudaMemcpyAsync(host, rt.ptr(v), nb, cudaMemcpyDeviceToHost, s));
     try {
+      GCHECK(cudaMemcpyAsync(host, rt.ptr(v), nb, cudaMemcpyDeviceToHost, s));
+      for (const auto& a : in_place) {
+        const gawee::Buf& b = rt.plan->bufs[rt.plan->arg_buf[a.first]];
+        GCHECK(cudaMemcpyAsync(a.second, b.ptr, b.bytes(), cudaMemcpyDeviceToHost, s));
+      }
       GCHECK(cudaStreamSynchronize(s));
       check_device_status(rt.d_status);
     } catch (...) {

@@ -59,6 +59,8 @@ def load_library(path: str = LIB_PATH):
             "gawee_set_arg": (c.c_int, [P, c.c_int, P, c.c_size_t, P]),
             "gawee_set_arg_device": (c.c_int, [P, c.c_int, P, c.c_size_t, P]),
             "gawee_arg_device_ptr": (c.c_int, [P, c.c_int, c.POINTER(P)]),
+            "gawee_arg_in_place": (c.c_int, [P, c.c_int]),
+            "gawee_get_arg": (c.c_int, [P, c.c_int, P, c.c_size_t, P]),
             "gawee_forward": (c.c_int, [P, P]),
             "gawee_get_output": (c.c_int, [P, c.c_int, P, c.c_size_t, P]),
             "gawee_output_device_ptr": (c.c_int, [P, c.c_int, c.POINTER(P)]),
@@ -136,6 +138,7 @@ class Model:
         self.arg_specs = [self._info(self._lib.gawee_arg_info, i) for i in range(self._lib.gawee_num_args(h))]
         self.output_specs = [self._info(self._lib.gawee_output_info, i)
                              for i in range(self._lib.gawee_num_outputs(h))]
+        self.in_place_args = [i for i in range(len(self.arg_specs)) if self._lib.gawee_arg_in_place(h, i) == 1]
 
     @classmethod
     def from_file(cls, path: str, **kw) -> "Model":
@@ -199,6 +202,18 @@ class Model:
         self._check(self._lib.gawee_arg_device_ptr(self._h, i, ctypes.byref(p)))
         return p.value
 
+    def arg(self, i: int, stream=None, out: Optional[np.ndarray] = None) -> np.ndarray:
+        """Argument i as the forwards left it; only one of `in_place_args`, the pages of paged_attention ops."""
+        dt, shape = self.arg_specs[i]
+        if out is None:
+            out = np.empty(shape, dtype=dt)
+        elif not out.flags.c_contiguous or out.dtype != dt:
+            raise GaweeError(1, f"argument {i} is read into a dense array of {dt}")
+        self._check(self._lib.gawee_get_arg(self._h, i, out.ctypes.data, out.nbytes, _stream_ptr(stream)))
+        if stream is None:
+            self.synchronize()
+        return out
+
     def set_args(self, arrays: Sequence[np.ndarray]):
         if len(arrays) != len(self.arg_specs):
             raise GaweeError(1, f"expected {len(self.arg_specs)} arguments, got {len(arrays)}")
@@ -227,10 +242,17 @@ class Model:
         return p.value
 
     def run(self, arrays: Sequence[np.ndarray]) -> List[np.ndarray]:
-        """Stage all arguments, run one forward, return every output (synchronous)."""
+        """Stage all arguments, run one forward, return every output (synchronous).
+        Arguments that the forward writes (`in_place_args`) are copied back into their arrays."""
+        for i in self.in_place_args:
+            if i < len(arrays) and not (isinstance(arrays[i], np.ndarray) and arrays[i].flags.c_contiguous
+                                        and arrays[i].flags.writeable):
+                raise GaweeError(1, f"argument {i} is written by the forward: it must be a writeable dense array")
         self.set_args(arrays)
         self.forward()
         self.synchronize()
+        for i in self.in_place_args:
+            self.arg(i, out=arrays[i])
         return [self.output(i) for i in range(len(self.output_specs))]
 
     def num_launches(self) -> int:

@@ -94,6 +94,13 @@ gawee_status gawee_set_arg_device(gawee_ctx* ctx, int i, const void* dev, size_t
  * packed weight is written with gawee_set_arg instead. */
 gawee_status gawee_arg_device_ptr(gawee_ctx* ctx, int i, void** ptr);
 
+/* Whether the forward writes argument i, as it does the pages of a
+ * gawee.paged_attention op: 1 or 0, -1 for an index out of range. */
+int gawee_arg_in_place(const gawee_ctx* ctx, int i);
+
+/* Copy an argument that the forward writes back to host memory (asynchronous on `stream`). */
+gawee_status gawee_get_arg(gawee_ctx* ctx, int i, void* host, size_t bytes, void* stream);
+
 /* Enqueue one forward on `stream`.  Replaces the call of
  * _mlir_ciface_forward (back/gawee_aot.cpp:263-274).  Asynchronous. */
 gawee_status gawee_forward(gawee_ctx* ctx, void* stream);
@@ -173,7 +180,10 @@ gawee_status gawee_plan_summary(const gawee_ctx* ctx, char* buf, size_t n);
  * malloc'ed buffer described by `result` (the callee allocates, as the
  * reference's lowered code does).  A memref descriptor is
  *   { T* allocated; T* aligned; int64_t offset; int64_t sizes[R]; int64_t strides[R]; }
- * and must describe a dense C-order array.
+ * and must describe a dense C-order array.  An argument that the forward
+ * writes (gawee_arg_in_place: the pages of a gawee.paged_attention op) is copied back
+ * into the caller's array, so that the next call has the rows which this one stored.
+ * A loop that keeps its pages on the device uses gawee_set_arg for what changes, and gawee_forward.
  * ------------------------------------------------------------------------- */
 gawee_status gawee_ciface_forward(gawee_ctx* ctx, void* result_desc, void* const* arg_descs, int nargs);
 
@@ -234,7 +244,10 @@ gawee_status gawee_matmul_f32_noalloc(const float* a, const float* b, float* c, 
  * In a graph, gawee.paged_attention(q, k, v, k_pages, v_pages, block_table,
  * lengths) <{scale}> is gawee_kv_attend with k and v: f32, the table and lengths i32,
  * the pages two function arguments that nothing else uses; they live in the context and
- * keep the stored rows from one forward to the next.
+ * keep the stored rows from one forward to the next, until gawee_set_arg replaces them.
+ * The calls that stage every argument from host memory (gawee_ciface_forward,
+ * gawee_embedded_forward, Model.run in Python) copy the pages back after the forward;
+ * the file contract of gawee-cuda-runner has no place for them.
  *
  * A gawee_kv handle holds the shapes and the scratch memory, allocated once;
  * one handle serves any number of layers.
