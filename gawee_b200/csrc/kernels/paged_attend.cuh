@@ -30,7 +30,7 @@
 //
 // Rows that the mask takes out, rows behind the length and rows of bad pages
 // are not loaded: their stage rows are filled with zeros and their score is
-// -inf, so that whatever memory holds there cannot reach the result.
+// -inf, so that whatever memory holds there, or the query, cannot reach the result.
 #pragma once
 
 #include <algorithm>
@@ -84,6 +84,9 @@ __device__ __forceinline__ float warp_max(float x) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
+// A key's score with its mask value added: -inf where that is -inf, also for a
+// query that is not finite, whose product with the zeros of the row is NaN.
+__device__ __forceinline__ float masked(float s, float add) { return add == -INFINITY ? -INFINITY : s; }
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -240,7 +243,7 @@ struct LaneTile {
       }
 #pragma unroll
       for (int o = kOwn / 2; o; o >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
-      s[g] += a;
+      s[g] = masked(s[g] + a, a);
       mx[g] = fmaxf(m[g], warp_max(s[g]));
       changed |= mx[g] != m[g];
     }
@@ -480,8 +483,8 @@ struct MmaTile {
       const float2 a = *reinterpret_cast<const float2*>(add + key);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        s[j][2 * r] = fmaf(s[j][2 * r], scale, a.x);
-        s[j][2 * r + 1] = fmaf(s[j][2 * r + 1], scale, a.y);
+        s[j][2 * r] = masked(fmaf(s[j][2 * r], scale, a.x), a.x);
+        s[j][2 * r + 1] = masked(fmaf(s[j][2 * r + 1], scale, a.y), a.y);
         mx[r] = fmaxf(mx[r], fmaxf(s[j][2 * r], s[j][2 * r + 1]));
       }
     }

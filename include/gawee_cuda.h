@@ -353,7 +353,7 @@ typedef struct {
  * each row's weights, summed over the query heads that share its key/value
  * head, are added: weights_out = weights + sum_h p_h (weights NULL: zeros);
  * columns from length on are not touched.
- *   - A mask value of -inf takes the row out, whatever its K and V hold.  Other
+ *   - A mask value of -inf takes the row out, whatever its K and V or the query hold.  Other
  *     values are added as they are: a mask of the lowest finite value is one.
  *     A sequence of length 0, or whose rows are all taken out, gives zeros.
  *     A mask value of +inf or NaN gives NaN.

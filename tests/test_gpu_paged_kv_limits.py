@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_paged_kv import T, U, Cache, _half_step, _reference, _run
+from tests.test_gpu_paged_kv import T, U, Cache, _check_attend, _half_step, _normal, _reference, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,46 @@ def test_attend_large_fp16_scores(heads, kv, dim):
     _run(c, heads, "f16", q_scale=60.0)
     _run(c, heads, "f16", q_scale=60.0, scale=-0.125)
     _run(c, heads, "f16", scale=0.0)
+
+
+# (pages, activations), heads, kv heads, head dim: fp32 lanes of one and two keys, of 4 to 32 lanes a row, and tensor cores
+FORMS = [("f32", "f32", 3, 3, 24), ("f32", "f32", 9, 3, 64), ("f32", "f32", 8, 1, 128), ("f32", "f32", 7, 1, 200),
+         ("bf16", "f32", 4, 1, 200), ("f16", "f32", 6, 2, 48), ("bf16", "bf16", 4, 2, 8), ("f16", "f16", 4, 2, 64),
+         ("bf16", "bf16", 16, 1, 64), ("bf16", "bf16", 8, 2, 128), ("f16", "f16", 12, 1, 96), ("bf16", "bf16", 8, 1, 256)]
+
+
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: "-".join(map(str, f)))
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_queries_that_are_not_finite_leave_masked_rows_out(form, value):
+    """Sequences whose rows are all taken out give zeros and no weights whatever
+    their queries hold, as the unused rows of a padded batch do; beside
+    attended rows such a query spoils its own head only."""
+    cache, act, heads, kv, dim = form
+    rng = np.random.default_rng(90)
+    lens = [3, 600, 70, 0, 90]
+    c = Cache(rng, lens, kv, dim, 16, cache)
+    n = c.cols * c.page
+    mask = torch.zeros(5, n)
+    mask[:2] = -float("inf")
+    mask[2, :40] = -float("inf")
+    q = _normal(rng, (5, heads, dim), act)
+    q[0] = q[3] = value
+    q[1, :, 1] = value
+    q[2, heads - 1, 2] = value
+    q, mask = q.cuda(), mask.cuda()
+    w = torch.rand((5, kv, n), device="cuda")
+    wo = torch.full_like(w, 5.0)
+    h = c.handle(heads, weights=True)
+    out = h.attend(c.k, c.v, q, c.table, c.lengths(), torch.full_like(q, 7.0), mask=mask, weights=w, weights_out=wo)
+    h.synchronize()
+    for i in (0, 1, 3):
+        assert (out[i] == 0).all(), f"sequence {i}"
+        assert torch.equal(wo[i, :, :lens[i]], w[i, :, :lens[i]])
+    assert not torch.isfinite(out[2, heads - 1].float()).all()
+    assert torch.isfinite(out[2, :heads - 1].float()).all() and torch.isfinite(out[4].float()).all()
+    assert torch.equal(wo[2, :, :40], w[2, :, :40])
+    c.lens = [-1, -1, -1, -1, 90]
+    out[:4] = 7
+    wo[:4] = 5
+    before = torch.full_like(w, 5.0)
+    _check_attend(c, q, out, act, dim ** -0.5, None, w, wo, before)
