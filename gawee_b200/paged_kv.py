@@ -33,7 +33,7 @@ _NAMES = {"float32": 0, "float16": 2, "bfloat16": 7, "int32": 4}
 _dtype_codes: dict = {}
 
 # The argument structures of include/gawee_cuda.h, packed with C alignment.
-_DESC = struct.Struct("@iiiiiqqiii")
+_DESC = struct.Struct("@iiiiiqqiii0q")  # 0q: the padding behind the last member
 _APPEND = struct.Struct("@PPPPiqqqPPPqii")
 _ATTEND = struct.Struct("@PPPPiqqifPqiPPPqqPqqPqqPqqq")
 _EVICT = struct.Struct("@PPPqqPqqqiPqiPqiPPiiP")
