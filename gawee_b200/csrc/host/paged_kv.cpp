@@ -336,7 +336,8 @@ gawee_status gawee_kv_evict(gawee_kv* kv, const gawee_kv_evict_args* a, void* st
     if (!kv || !a) return bad("null handle or arguments");
     std::string m = check_common(kv, a->k_pages, a->v_pages, a->batch, a->block_table, a->table_stride, a->table_cols);
     if (!m.empty()) return bad(m);
-    if (a->budget < 1) return bad("budget is below 1");
+    // the kernels step past the last kept row by less than 2^24
+    if (a->budget < 1 || a->budget > INT32_MAX - (1 << 24)) return bad("budget is below 1, or 2^31 - 2^24 or more");
     if (a->recent < 0 || a->recent > a->budget) return bad("recent outside 0 .. budget");
     if (a->batch == 0) return GAWEE_OK;
     if (!a->weights || !a->weights_out || !a->lengths || !a->lengths_out || !a->kept)

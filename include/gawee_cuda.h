@@ -382,7 +382,7 @@ typedef struct {
   int to_cols;
   const int32_t* lengths;
   int32_t* lengths_out; /* may be `lengths` itself */
-  int budget;           /* rows that a sequence keeps at most, at least 1 */
+  int budget;           /* rows that a sequence keeps at most: at least 1, below 2^31 - 2^24 */
   int recent;           /* of these, the last rows that always stay, 0 .. budget */
   int32_t* kept;        /* [batch][kv_heads][budget]: earlier positions of the kept rows, ascending; -1 behind them */
 } gawee_kv_evict_args;

@@ -2,7 +2,9 @@
 import os
 import subprocess
 
-from gawee_b200 import build, paged_kv
+import pytest
+
+from gawee_b200 import build, paged_kv, runtime
 
 STRUCTS = {"gawee_kv_desc": paged_kv._DESC, "gawee_kv_append_args": paged_kv._APPEND,
            "gawee_kv_attend_args": paged_kv._ATTEND, "gawee_kv_evict_args": paged_kv._EVICT}
@@ -17,3 +19,15 @@ def test_packed_arguments_are_as_long_as_the_structures(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-I", os.path.join(build.ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [s.size for s in STRUCTS.values()]
+
+
+@pytest.mark.parametrize("budget,status", [(0, 1), (-1, 1), (1, 4), ((1 << 31) - (1 << 24) - 1, 4), ((1 << 31) - (1 << 24), 1),
+                                           ((1 << 31) - 1, 1)])
+def test_evict_refuses_budgets_that_the_kernels_indices_would_pass(budget, status):
+    """A handle without a device: 1 is a refused argument, 4 the missing device behind the checks.
+    A block of the move goes on by 16 x 148 blocks of up to 1024 rows, in 32 bits."""
+    kv = paged_kv.PagedKV("bf16", 2, 1, 8, 16, 64, 4, 8, device=-1)
+    some = 1 << 20  # an address that nothing reads
+    packed = paged_kv._EVICT.pack(some, 2 * some, some, 64, 64, some, 64, 64, 64, 2, some, 8, 8, 0, 0, 0, some, some, budget,
+                                  0, some)
+    assert runtime.load_library().gawee_kv_evict(kv._h, packed, None) == status
