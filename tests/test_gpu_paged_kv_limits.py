@@ -106,3 +106,29 @@ def test_queries_that_are_not_finite_leave_masked_rows_out(form, value):
     wo[:4] = 5
     before = torch.full_like(w, 5.0)
     _check_attend(c, q, out, act, dim ** -0.5, None, w, wo, before)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: "-".join(map(str, f)))
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_mask_value_of_nan_or_infinity_gives_nan(form, value):
+    """In its own sequence only, wherever it lies: in the first, a middle or the last row of one or of many tiles."""
+    cache, act, heads, kv, dim = form
+    rng = np.random.default_rng(91)
+    lens = [1, 700, 30, 2500, 45]
+    c = Cache(rng, lens, kv, dim, 16, cache)
+    n = c.cols * c.page
+    mask = torch.zeros(5, n)
+    for i, at in ((0, 0), (1, 0), (2, 17), (3, 2499)):
+        mask[i, at] = value
+    mask[2, :17] = -float("inf")
+    q = _normal(rng, (5, heads, dim), act).cuda()
+    h = c.handle(heads, weights=True)
+    wo = torch.full((5, kv, n), 5.0, device="cuda")
+    before = wo.clone()
+    out = h.attend(c.k, c.v, q, c.table, c.lengths(), torch.full_like(q, 7.0), mask=mask.cuda(), weights_out=wo)
+    h.synchronize()
+    assert torch.isnan(out[:4].float()).all()
+    out[:4] = 7
+    wo[:4] = 5
+    c.lens = [-1, -1, -1, -1, 45]
+    _check_attend(c, q, out, act, dim ** -0.5, None, None, wo, before)
