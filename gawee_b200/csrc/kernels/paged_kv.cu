@@ -379,8 +379,10 @@ __global__ void __launch_bounds__(THREADS) kv_select_kernel(KvEvictParams p) {
           const uint32_t k = weight_key(x[r]);
           if (i < old_end && (k & upto) == prefix) {
             const int at = atomicAdd(&s_left, 1);
-            s_key[at] = k;
-            s_at[at] = i;
+            if (at < THREADS) {  // more of them only if the weights change meanwhile
+              s_key[at] = k;
+              s_at[at] = i;
+            }
           }
         }
       }
@@ -459,7 +461,8 @@ __global__ void __launch_bounds__(THREADS) kv_select_kernel(KvEvictParams p) {
     int s = sure_before + (before & 0xffff), q = equal_before + (before >> 16);
 #pragma unroll
     for (int x = 0; x < kEach; ++x) {
-      if (a[x] || (e[x] && q < need)) kept[s + min(q, need)] = base + tid * kEach + x;
+      const int place = s + min(q, need);
+      if ((a[x] || (e[x] && q < need)) && place < p.budget) kept[place] = base + tid * kEach + x;
       s += a[x];
       q += e[x];
     }
@@ -477,6 +480,10 @@ __global__ void __launch_bounds__(THREADS) kv_select_kernel(KvEvictParams p) {
 // each step's rows after the whole step is read; slices are as narrow as it
 // takes to occupy the GPU.  The last block of a pair moves its weights.  Bound by
 // HBM: 256 pairs, up to 2048 rows of 256 bytes each, to other pages: 95 us, 5.2 TB/s.
+//
+// Calls that overlap against the rule exchange their `plan`, and weights that
+// change during a call its selection: every position is checked before it is
+// used, so that they spoil no more than the results.
 constexpr int kMoveThreads = 256, kMoveRows = 4;  // rows of a thread in a step
 
 template <bool IN_PLACE>
@@ -503,7 +510,8 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(KvEvictParams p, 
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         const int j = j0 + e * kMoveThreads + tid;
-        x[e] = j < left ? w[kept[j]] : 0.f;
+        const int src = j < left ? kept[j] : -1;
+        x[e] = src >= 0 && src < len ? w[src] : 0.f;
       }
       __syncthreads();  // read before they are written over
 #pragma unroll

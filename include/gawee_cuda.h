@@ -263,6 +263,8 @@ gawee_status gawee_matmul_f32_noalloc(const float* a, const float* b, float* c, 
  *     that may run at the same time take a handle each.  (Nothing of one call
  *     stays in the scratch for the next: calls that overlap against this rule
  *     spoil their own results, and no later ones.)
+ *   - What a call reads (lengths, tables, positions, weights) is not written by
+ *     others while it runs.
  *   - A bad argument is refused with GAWEE_ERR_INVALID before anything is
  *     enqueued; the message is read with gawee_last_error(NULL, ...).
  *   - What only the device can see (a table entry that names no page, a length

@@ -132,3 +132,61 @@ def test_a_mask_value_of_nan_or_infinity_gives_nan(form, value):
     wo[:4] = 5
     c.lens = [-1, -1, -1, -1, 45]
     _check_attend(c, q, out, act, dim ** -0.5, None, None, wo, before)
+
+
+def test_evictions_that_overlap_on_one_handle_spoil_no_later_one():
+    """Two streams without an order, one handle: lengths and budgets differ, so
+    that each call may find the other's plan.  Their own results are lost; what
+    lies around their arrays, and the calls after them, are not."""
+    rng = np.random.default_rng(92)
+    kv, dim, page, batch = 2, 16, 16, 6
+
+    def case(lens, budget, seed):
+        c = Cache(np.random.default_rng(seed), lens, kv, dim, page, "bf16")
+        n = c.cols * page
+        around = torch.full((batch * kv * n + 64,), 3.0, device="cuda")  # weights with a margin on both sides
+        w = around[32:-32].view(batch, kv, n)
+        w.copy_(torch.from_numpy(rng.random((batch, kv, n), dtype=np.float32)))
+        kept = torch.full((batch * kv * budget + 64,), 55, dtype=torch.int32, device="cuda")
+        return dict(c=c, w=w, lens=c.lengths(), budget=budget, kept=kept[32:-32].view(batch, kv, budget), around=around,
+                    kept_around=kept, lens_out=torch.zeros(batch, dtype=torch.int32, device="cuda"))
+
+    def evict(h, x, stream=None):
+        h.evict(x["c"].k, x["c"].v, x["w"], x["c"].table, x["lens"], x["budget"], 5, x["kept"], x["w"], x["lens_out"],
+                stream=stream)
+
+    few, many = [1, 0, 3, -1, 2, 5], [900, 700, 33, 2000, -1, 1500]
+    cases = [case(few, 400, 1), case(many, 40, 2)]
+    cases[0]["c"].num_pages = cases[1]["c"].num_pages = max(x["c"].num_pages for x in cases)
+    for x in cases:  # pages of one shape, for one handle
+        for name in ("k", "v"):
+            p = torch.zeros((x["c"].num_pages,) + getattr(x["c"], name).shape[1:], dtype=torch.bfloat16, device="cuda")
+            p[:getattr(x["c"], name).shape[0]] = getattr(x["c"], name)
+            setattr(x["c"], name, p)
+    h = cases[1]["c"].handle(kv, max_pages=200)
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(40):
+        for x, s in zip(cases, streams):
+            evict(h, x, s)
+    torch.cuda.synchronize()
+    try:
+        h.synchronize()  # a spoilt call may have found a position without a page
+    except Exception as e:
+        assert "device reported" in str(e)
+    for x in cases:
+        for margin, value in ((x["around"], 3), (x["kept_around"], 55)):
+            assert (margin[:32] == value).all() and (margin[-32:] == value).all()
+    # the same handle again, in order, and a new one
+    again, fresh = case(many, 40, 3), case(many, 40, 3)
+    fresh["w"].copy_(again["w"])
+    h2 = fresh["c"].handle(kv, max_pages=200)
+    assert again["c"].num_pages == cases[1]["c"].num_pages
+    evict(h, again)
+    evict(h2, fresh)
+    h.synchronize()
+    h2.synchronize()
+    for name in ("kept", "w", "lens_out"):
+        assert torch.equal(again[name], fresh[name]), name
+    assert torch.equal(torch.nan_to_num(again["c"].k), torch.nan_to_num(fresh["c"].k))
+    assert again["lens_out"].tolist() == [40, 40, 33, 40, -1, 40]
