@@ -953,7 +953,8 @@ __global__ void __launch_bounds__(kThreads, P::kMinBlocks) kv_attend_kernel(cons
         first += TILE;
         if (p.weights_out) scores += (long long)TILE * group;
       }
-      // the warp's state takes the place of the stage it has just used
+      // the warp's state takes the place of the stage it has just used: every lane has read its V rows
+      __syncwarp();
       state.dump(&s_ml[warp][0][0], reinterpret_cast<float*>(ring + stage_at));
     }
     j += mine;

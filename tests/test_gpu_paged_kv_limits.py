@@ -190,3 +190,19 @@ def test_evictions_that_overlap_on_one_handle_spoil_no_later_one():
         assert torch.equal(again[name], fresh[name]), name
     assert torch.equal(torch.nan_to_num(again["c"].k), torch.nan_to_num(fresh["c"].k))
     assert again["lens_out"].tolist() == [40, 40, 33, 40, -1, 40]
+
+
+@pytest.mark.parametrize("form", [("f32", "f32", 8, 1, 200), ("f32", "f32", 14, 2, 256), ("bf16", "f32", 4, 1, 200),
+                                  ("f16", "f32", 8, 2, 256), ("f32", "bf16", 6, 1, 136)], ids=lambda f: "-".join(map(str, f)))
+def test_long_rows_give_the_same_bits_again(form):
+    """Rows of more than 128 elements, whose partial sums take the place of the
+    values that the last tile of a segment held: many segments of a few tiles."""
+    cache, act, heads, kv, dim = form
+    rng = np.random.default_rng(93)
+    c = Cache(rng, [int(x) for x in rng.integers(1, 150, 120)], kv, dim, 16, cache)
+    h = c.handle(heads)
+    first = _run(c, heads, act, kv=h)
+    q = _normal(np.random.default_rng(3), (120, heads, dim), act, 2.0).cuda()
+    outs = [h.attend(c.k, c.v, q, c.table, c.lengths(), torch.empty_like(q)) for _ in range(10)]
+    h.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
