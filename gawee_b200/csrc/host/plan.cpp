@@ -1901,7 +1901,10 @@ class Planner {
     if (B > 65535 || H > 4096 || ps[0] > INT32_MAX || table.shape[1] * ps[2] > INT32_MAX - (1 << 20))
       unsupported("paged_attention: batch, heads, pages or rows beyond the limits of gawee_kv_create");
     const Attr& sc = n.attr("scale");
+    if (sc.kind != Attr::INT && sc.kind != Attr::FLOAT) unsupported("paged_attention: scale is not a number");
     const double scale = sc.kind == Attr::INT ? (double)sc.i : sc.f;
+    if (!std::isfinite((float)scale)) unsupported("paged_attention: scale is not finite in f32");
+    if (val(n.outs[0]).type.dtype != DType::F32) unsupported("paged_attention: the result is f32");
     View out = alloc(DType::F32, val(n.outs[0]).type.shape);
     if (out.shape != q.shape) unsupported("paged_attention: the result has q's shape");
     View parts = alloc(DType::F32, {kern::kv_parts_floats(kern::kKvPlanSms, (int)(H / KV), (int)D)});

@@ -5,6 +5,7 @@ import subprocess
 import pytest
 
 from gawee_b200 import build, paged_kv, runtime
+from tests.test_paged_kv import _op_graph
 
 STRUCTS = {"gawee_kv_desc": paged_kv._DESC, "gawee_kv_append_args": paged_kv._APPEND,
            "gawee_kv_attend_args": paged_kv._ATTEND, "gawee_kv_evict_args": paged_kv._EVICT}
@@ -31,3 +32,20 @@ def test_evict_refuses_budgets_that_the_kernels_indices_would_pass(budget, statu
     packed = paged_kv._EVICT.pack(some, 2 * some, some, 64, 64, some, 64, 64, 64, 2, some, 8, 8, 0, 0, 0, some, some, budget,
                                   0, some)
     assert runtime.load_library().gawee_kv_evict(kv._h, packed, None) == status
+
+
+@pytest.mark.parametrize("old,new", [
+    ("scale = 0.5 : f64", "scale = 1.0e39 : f64"), ("scale = 0.5 : f64", "scale = -1.0e400 : f64"),
+    ("scale = 0.5 : f64", "scale = true"), ("scale = 0.5 : f64", 'scale = "0.5"'), ("scale = 0.5 : f64", "scale = [0.5]"),
+    ("-> tensor<3x6x16xf32>\n    return", "-> tensor<3x6x16xf16>\n    return"),
+])
+def test_graph_op_refuses_a_scale_that_is_no_finite_number_and_other_results(old, new):
+    """gawee_kv_attend refuses such a scale too; taken as it was, it became 0 or infinity."""
+    text = _op_graph()
+    for scale in ("0.5 : f64", "-2 : i64", "0.0 : f32"):
+        assert "paged_attention" in runtime.plan_text(text.replace("0.5 : f64", scale))
+    assert text.count(old) == 1
+    text = text.replace(old, new)
+    with pytest.raises(runtime.GaweeError, match="paged_attention"):
+        runtime.plan_text(text.replace("return %0 : tensor<3x6x16xf32>", "return %0 : tensor<3x6x16xf16>")
+                          if "f16" in new else text)
