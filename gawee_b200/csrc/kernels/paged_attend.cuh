@@ -42,7 +42,7 @@ namespace gawee {
 namespace kern {
 namespace paged {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = kKvWarps;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBlocksPerSm = kKvMaxBlocksPerSm;
 constexpr int kMaxSmem = 220 * 1024;  // of a block, beside the kernel's static variables
@@ -109,8 +109,8 @@ template <class T_, int L, int NH_, bool FULL>
 struct LaneTile {
   using T = T_;
   static constexpr int NH = NH_;
-  static constexpr int kKeysAtOnce = 32 / L, kSteps = 4;
-  static constexpr int TK = kSteps * kKeysAtOnce;  // keys of a warp's tile
+  static constexpr int TK = kv_warp_keys(L);  // keys of a warp's tile
+  static constexpr int kKeysAtOnce = 32 / L, kSteps = TK / kKeysAtOnce;
   // Lanes that share a key, and the keys that they take at once: two for long
   // fp32 rows and several heads, where the reads of the queries would fill shared
   // memory's time (8 heads x 128, 74,862 rows: 74 us, with one key 84; in 16 bits
@@ -1063,12 +1063,14 @@ cudaError_t attend_lanes_group(const KvAttendParams& p, KvAttendShape* shape, cu
 template <class T>
 cudaError_t attend_lanes(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
   const int D = p.geom.head_dim;
-  if (D <= 32) return attend_lanes_group<T, 4, false>(p, shape, s);
-  if (D < 64) return attend_lanes_group<T, 8, false>(p, shape, s);
-  if (D == 64) return attend_lanes_group<T, 8, true>(p, shape, s);
-  if (D < 128) return attend_lanes_group<T, 16, false>(p, shape, s);
-  if (D == 128) return attend_lanes_group<T, 16, true>(p, shape, s);
-  return attend_lanes_group<T, 32, false>(p, shape, s);
+  switch (kv_row_lanes(D)) {
+    case 4: return attend_lanes_group<T, 4, false>(p, shape, s);
+    case 8:
+      return D == 64 ? attend_lanes_group<T, 8, true>(p, shape, s) : attend_lanes_group<T, 8, false>(p, shape, s);
+    case 16:
+      return D == 128 ? attend_lanes_group<T, 16, true>(p, shape, s) : attend_lanes_group<T, 16, false>(p, shape, s);
+    default: return attend_lanes_group<T, 32, false>(p, shape, s);
+  }
 }
 template <class T, int NH>
 cudaError_t attend_mma(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {

@@ -25,10 +25,15 @@ inline int64_t kv_parts_floats(int sms, int group, int head_dim) {
 }
 inline int64_t kv_blocks(int sms) { return (int64_t)sms * kKvMaxBlocksPerSm; }
 inline int64_t kv_segments(int64_t batch, int kv_heads, int group) { return batch * kv_heads * ((group + 3) / 4); }
+// Attention by fp32 lanes: the lanes that hold a row, and the keys of a warp's
+// tile (paged_attend.cuh, which is instantiated by these).
+constexpr int kKvWarps = 4;
+constexpr int kv_row_lanes(int head_dim) { return head_dim <= 32 ? 4 : head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32; }
+constexpr int kv_warp_keys(int row_lanes) { return 128 / row_lanes; }
 // Launches of an attention over f32 pages without weights: a second one joins
-// the parts where a sequence may be longer than a tile (paged_attend.cuh: 128 / L keys a warp).
+// the parts where a sequence may be longer than a block's tile.
 inline int kv_attend_launches_f32(int head_dim, int64_t max_len) {
-  return max_len > (head_dim <= 32 ? 128 : head_dim <= 64 ? 64 : head_dim <= 128 ? 32 : 16) ? 2 : 1;
+  return max_len > kKvWarps * kv_warp_keys(kv_row_lanes(head_dim)) ? 2 : 1;
 }
 // SMs that a graph's workspace is planned for; a GPU with more uses this many.
 constexpr int kKvPlanSms = 160;

@@ -49,3 +49,27 @@ def test_graph_op_refuses_a_scale_that_is_no_finite_number_and_other_results(old
     with pytest.raises(runtime.GaweeError, match="paged_attention"):
         runtime.plan_text(text.replace("return %0 : tensor<3x6x16xf32>", "return %0 : tensor<3x6x16xf16>")
                           if "f16" in new else text)
+
+
+def test_the_lane_forms_and_their_launches_go_by_one_rule(tmp_path):
+    """Which lane form a head dim takes and how many launches a call makes, compiled for the host."""
+    src = tmp_path / "r.cpp"
+    src.write_text("""
+#include <cassert>
+#include "paged_kv.h"
+using namespace gawee::kern;
+int main() {
+  for (int d = 8; d <= 256; d += 8) {
+    const int lanes = kv_row_lanes(d), tile = kKvWarps * kv_warp_keys(lanes);
+    assert(8 * lanes >= d && (lanes == 4 || 4 * lanes < d));  // eight elements a lane hold a row, half as many lanes do not
+    assert(tile == (d <= 32 ? 128 : d <= 64 ? 64 : d <= 128 ? 32 : 16));
+    assert(kv_attend_launches_f32(d, 1) == 1 && kv_attend_launches_f32(d, tile) == 1);
+    assert(kv_attend_launches_f32(d, tile + 1) == 2 && kv_attend_launches_f32(d, 1ll << 40) == 2);
+  }
+}
+""")
+    exe = tmp_path / "r"
+    cuda = os.path.join(os.path.dirname(os.path.dirname(build.nvcc())), "include")
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(build.CSRC, "kernels"), "-I", cuda, str(src), "-o", str(exe)],
+                   check=True)
+    subprocess.run([str(exe)], check=True)
