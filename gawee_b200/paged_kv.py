@@ -213,10 +213,13 @@ class PagedKV:
             wp, ws, wb, c = self._weights(weights, "weights", batch)
             if weights_out is not None and c != wc:
                 raise _invalid(f"weights has {c} columns, weights_out {wc}")
-        a = _ATTEND.pack(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), qp, op, code, qs, os_, batch,
-                         self.head_dim ** -0.5 if scale is None else scale, tp, ts, cols,
-                         self._ints(lengths, "lengths", batch), kp, vp, ks, vs, mp, ms, mc, wp, ws, wb, wop, wos, wob,
-                         wc)
+        try:
+            a = _ATTEND.pack(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), qp, op, code, qs, os_,
+                             batch, self.head_dim ** -0.5 if scale is None else scale, tp, ts, cols,
+                             self._ints(lengths, "lengths", batch), kp, vp, ks, vs, mp, ms, mc, wp, ws, wb, wop, wos,
+                             wob, wc)
+        except (struct.error, OverflowError) as e:  # a value that its C type cannot hold
+            raise _invalid(f"scale is {scale!r}: {e}") from None
         self._check(self._lib.gawee_kv_attend(self._h, a, _stream_ptr(stream)))
         return out
 
@@ -241,10 +244,13 @@ class PagedKV:
             top, tos, rows, toc = self._table(to_table, "to_table")
             if rows != batch:
                 raise _invalid(f"to_table has {rows} rows, block_table {batch}")
-        a = _EVICT.pack(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), wp, ws, wb, wop, wos, wob, wc,
-                        batch, tp, ts, cols, top, tos, toc, self._ints(lengths, "lengths", batch),
-                        self._ints(lengths_out, "lengths_out", batch), budget, recent,
-                        self._on_device(kept, "kept", 4))
+        try:
+            a = _EVICT.pack(self._pages(k_pages, "k_pages"), self._pages(v_pages, "v_pages"), wp, ws, wb, wop, wos, wob,
+                            wc, batch, tp, ts, cols, top, tos, toc, self._ints(lengths, "lengths", batch),
+                            self._ints(lengths_out, "lengths_out", batch), budget, recent,
+                            self._on_device(kept, "kept", 4))
+        except struct.error as e:
+            raise _invalid(f"budget is {budget!r}, recent {recent!r}: {e}") from None
         self._check(self._lib.gawee_kv_evict(self._h, a, _stream_ptr(stream)))
 
     def synchronize(self, stream=None):

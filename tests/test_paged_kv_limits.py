@@ -5,7 +5,7 @@ import subprocess
 import pytest
 
 from gawee_b200 import build, paged_kv, runtime
-from tests.test_paged_kv import _op_graph
+from tests.test_paged_kv import _attend_args, _evict_args, _handle, _op_graph
 
 STRUCTS = {"gawee_kv_desc": paged_kv._DESC, "gawee_kv_append_args": paged_kv._APPEND,
            "gawee_kv_attend_args": paged_kv._ATTEND, "gawee_kv_evict_args": paged_kv._EVICT}
@@ -73,3 +73,15 @@ int main() {
     subprocess.run(["g++", "-std=c++17", "-I", os.path.join(build.CSRC, "kernels"), "-I", cuda, str(src), "-o", str(exe)],
                    check=True)
     subprocess.run([str(exe)], check=True)
+
+
+@pytest.mark.parametrize("call,kw", [
+    ("attend", dict(scale=1e39)), ("attend", dict(scale=-1e300)), ("attend", dict(scale="0.5")),
+    ("attend", dict(scale=1 << 2000)), ("evict", dict(budget=6.0)), ("evict", dict(recent=1.5)),
+])
+def test_numbers_that_their_c_type_cannot_hold_are_refused_like_other_arguments(call, kw):
+    kv = _handle()
+    args = (_attend_args if call == "attend" else _evict_args)(**kw)
+    with pytest.raises(runtime.GaweeError) as e:
+        getattr(kv, call)(**args)
+    assert e.value.status == 1 and next(iter(kw)) in str(e.value)
