@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_paged_kv import T, U, Cache, _check_attend, _half_step, _normal, _reference, _run
+from tests.test_gpu_paged_kv import T, U, Cache, _check_attend, _half_step, _kv, _normal, _reference, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -206,3 +206,68 @@ def test_long_rows_give_the_same_bits_again(form):
     outs = [h.attend(c.k, c.v, q, c.table, c.lengths(), torch.empty_like(q)) for _ in range(10)]
     h.synchronize()
     assert all(torch.equal(o, first) for o in outs)
+
+
+@pytest.mark.parametrize("types", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32")],
+                         ids=lambda t: f"{t[0]}-{t[1]}")
+@pytest.mark.parametrize("group", [1, 3, 5, 11])
+def test_every_head_dim(types, group):
+    """All multiples of 8 up to 256, the new row stored and weights added: ends inside and at the end of tiles and pages."""
+    for dim in range(8, 257, 8):
+        c = Cache(np.random.default_rng(dim), [1, 31, 32, 140, 65], 2, dim, (16, 7, 33)[dim // 8 % 3], types[0])
+        _run(c, 2 * group, types[1], seed=dim + group, new=True, with_weights=True)
+
+
+@pytest.mark.parametrize("types,dim", [(("bf16", "bf16"), 16), (("f16", "f16"), 64), (("f32", "f32"), 8), (("bf16", "f32"), 8)],
+                         ids=lambda v: "-".join(v) if isinstance(v, tuple) else str(v))
+def test_attend_the_longest_sequence(types, dim):
+    """2^31 - 2^20 - 1024 rows, whose table names one page again and again.
+
+    Keys of zeros make every weight 1, and values of 0 and 1 every sum of a block
+    a whole number below 2^24, so exact.  A sum of the blocks' parts, of at most
+    592 blocks, and the division round 600 times at most: 2 * 600 u relatively.
+    """
+    page = 1024
+    cols = (1 << 21) - 1025
+    k = torch.zeros((2, 1, page, dim), dtype=T[types[0]], device="cuda")
+    v = torch.full_like(k, float("nan"))
+    ones = torch.arange(page)[:, None] * (torch.arange(dim)[None] + 1) % 3 == 0
+    v[1, 0] = ones.cuda().to(T[types[0]])
+    table = torch.ones((1, cols), dtype=torch.int32, device="cuda")
+    from gawee_b200.paged_kv import PagedKV
+    h = PagedKV(types[0], 2, 1, dim, page, 2, 1, cols)
+    q = torch.ones((1, 2, dim), dtype=T[types[1]], device="cuda")
+    lens = torch.tensor([cols * page], dtype=torch.int32, device="cuda")
+    out = h.attend(k, v, q, table, lens, torch.empty_like(q))
+    h.synchronize()
+    want = ones.double().mean(0).expand(2, dim)
+    tol = want * (1200 * U + _half_step(types[1])) + 1e-30
+    err = (out[0].cpu().double() - want).abs()
+    assert (err <= tol).all(), f"off by {(err / tol).max():.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("types", [("f32", "f32"), ("bf16", "bf16")], ids=lambda t: f"{t[0]}-{t[1]}")
+def test_the_largest_batch_and_the_largest_group(types):
+    """65,535 sequences of a few rows or none; 4096 query heads over one key/value head."""
+    rng = np.random.default_rng(94)
+    lens = [int(x) for x in rng.choice([-1, 0, 1, 2, 9], 65535)]
+    c = Cache(rng, [1], 1, 8, 4, types[0])  # one page, of which every sequence reads the first rows
+    c.k.nan_to_num_(nan=0.5)
+    c.v = _normal(rng, c.v.shape, types[0]).cuda()
+    h = _kv(types[0], 2, 1, 8, 4, c.num_pages, max_batch=65535, max_pages=3, weights=True)
+    table = torch.randint(0, c.num_pages, (65535, 3), dtype=torch.int32, device="cuda")
+    q = _normal(rng, (65535, 2, 8), types[1]).cuda()
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    wo = torch.full((65535, 1, 12), 5.0, device="cuda")
+    out = h.attend(c.k, c.v, q, table, lengths, torch.full_like(q, 7.0), weights_out=wo)
+    h.synchronize()
+    # the same in smaller batches, whose results the other tests hold against the formula
+    small = _kv(types[0], 2, 1, 8, 4, c.num_pages, max_batch=1000, max_pages=3, weights=True)
+    for at in range(0, 65535, 1000):
+        part = slice(at, min(at + 1000, 65535))
+        w1 = torch.full_like(wo[part], 5.0)
+        o1 = small.attend(c.k, c.v, q[part], table[part], lengths[part], torch.full_like(q[part], 7.0), weights_out=w1)
+        assert torch.equal(out[part], o1) and torch.equal(wo[part], w1), at
+    small.synchronize()
+    wide = Cache(rng, [300, 5], 1, 16, 16, types[0])
+    _run(wide, 4096, types[1], with_weights=True, new=True)
