@@ -25,7 +25,8 @@
 // Measured, with the join, in a captured graph: 32 sequences of up to 8192 rows,
 // 32/8 heads x 128, bf16: 103 us, 5.8 TB/s, 0.88 of the copy rate; one of 131,071
 // rows: 87 us, 6.2 TB/s; 64 of up to 2048 rows, 9/3 heads x 64, fp32: 30 us,
-// 3.7 TB/s, bound by instruction issue; one of 257 rows, 6 heads x 48: 8 us, a
+// 3.7 TB/s, bound by latency: three warps a scheduler that wait for loads and for each
+// other use 39 % of the issue slots and 57 % of DRAM; one of 257 rows, 6 heads x 48: 8 us, a
 // chain of lookups.
 //
 // Rows that the mask takes out, rows behind the length and rows of bad pages
@@ -113,13 +114,14 @@ struct LaneTile {
   static constexpr int kKeysAtOnce = 32 / L, kSteps = TK / kKeysAtOnce;
   // Lanes that share a key, and the keys that they take at once: two for long
   // fp32 rows and several heads, where the reads of the queries would fill shared
-  // memory's time (8 heads x 128, 74,862 rows: 74 us, with one key 84; in 16 bits
-  // with 4 heads one key is the faster, 51 against 52).
+  // memory's time (one of 65,536 rows, 32/4 heads x 128: 69 us, with one key 77; 8 of up to
+  // 8192, 32/8 heads: 44.0, 44.6).  Over 16-bit rows one key is the faster (one of 65,536
+  // rows, 16/4 heads x 128, bf16 pages: 47.2 us, with two 48.4).
   static constexpr int KL = sizeof(T) == 4 && L >= 16 && NH >= 4 ? 2 : 1;
   static constexpr int W = 32 * KL / TK, kOwn = W / KL;  // kOwn lanes end up with the same key
   // With two stages three blocks find room on an SM, with about 96 KB on the
-  // way; twelve warps hide each other's waits better than eight with a third stage (b64
-  // of 9/3 x 64 heads, fp32: 52 us with three stages, 37 with two).
+  // way; twelve warps hide each other's waits better than eight with a third stage (64 of
+  // up to 2048 rows, 9/3 x 64 heads, fp32: 29.8 us, with three stages 30.8).
   static constexpr int kStages = (NH <= 6 ? 2 : 3) * (sizeof(T) == 4 ? 1 : 2);
   static constexpr int kMinBlocks = NH <= 6 ? 3 : 2;  // of an SM: what the stages leave room for
   static constexpr int kPer = 16 / sizeof(T);         // elements of a chunk
@@ -594,8 +596,8 @@ __device__ __forceinline__ int tiles_of(int len) {  // an empty sequence takes o
 // Units of work of a segment: `start` for its begin and end, then one a tile;
 // tile i is done by the block that has unit i + start.  With four tiles a block
 // and more the begin counts as two (9/3 x 64 heads, 64 sequences of up to 2048
-// rows, fp32: 30.4 us against 32.0); with fewer as one, or blocks that hold
-// nothing else would stand idle (one of 16,385 rows: 14.4 us against 16.1).
+// rows, fp32: 29.6 us against 30.4); with fewer as one, or blocks that hold
+// nothing else would stand idle (one of 16,385 rows: 14.3 us against 15.9).
 template <int TILE>
 __device__ __forceinline__ int units_of(int len, int start) {
   return len < 0 ? 0 : tiles_of<TILE>(len) + start;
@@ -1084,10 +1086,11 @@ cudaError_t attend_mma(const KvAttendParams& p, KvAttendShape* shape, cudaStream
 template <class T>
 cudaError_t attend_16bit(const KvAttendParams& p, KvAttendShape* shape, cudaStream_t s) {
   // Tensor cores need one type, and pay from 16 to 128 elements a row whatever the
-  // group (64 sequences of up to 1024 rows, 8 heads: 31.5 -> 21.2 us at 32
-  // elements, 36.4 -> 33.9 at 128); rows of 8 are mostly padding (18.0 -> 20.7) and longer ones leave an SM
-  // one block (192: 82 -> 118), which only the arithmetic of three heads and more
-  // outweighs (256 elements, 4 heads a key/value head, 74,862 rows: 132 -> 80).
+  // group.  bf16, 64 sequences of up to 1024 rows, 8/8 heads, lanes -> tensor cores:
+  // 16 elements 30.9 -> 24.0 us, 32 33.5 -> 23.2, 64 24.1 -> 24.0, 128 36.5 -> 34.3.
+  // Rows of 8 are mostly padding (17.9 -> 23.1) and longer ones leave an SM one block
+  // (192: 84.5 -> 107; two heads a key/value head: 104.5 -> 109), which only the arithmetic
+  // of three heads and more outweighs (12/4 heads of 256, one of 65,536 rows: 110 -> 73).
   const int D = p.geom.head_dim, group = p.heads / p.geom.kv_heads;
   if (p.dt == TypeCode<T>::value && ((D >= 16 && D <= 128) || group > 2))
     return group <= 8 ? attend_mma<T, 8>(p, shape, s) : attend_mma<T, 16>(p, shape, s);

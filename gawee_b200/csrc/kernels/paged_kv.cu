@@ -17,9 +17,10 @@ namespace {
 
 // --- append -------------------------------------------------------------------
 // A thread takes 16-byte vectors of a token's row over the heads, of K and of V.
-// The bound is HBM bandwidth; the chain position -> page -> row is short, and
-// many tokens are on the way at once.  13,786 tokens of 8 x 128, fp32 to bf16
-// pages of 16 rows: 35 us, 4.8 TB/s (an element a thread: 68 us); 63 tokens: 2.2 us.
+// The floor is HBM bandwidth; many tokens are on the way at once, but a block's work
+// is short and begins with the chain sequence and position -> page -> row.
+// 13,786 tokens of 8 x 128, fp32 to bf16 pages of 16 rows: 35 us, 4.8 TB/s, 0.73 of
+// the copy rate (an element a thread: 68 us); 63 tokens: 2.2 us.
 constexpr int kAppendThreads = 256;
 
 // `n` consecutive values as fp32; 16-byte loads where the caller knows the alignment.
@@ -93,8 +94,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendParam
 // head: the parts' maxima and sums give each part's factor, and groups of
 // threads add the scaled parts, in a fixed order.  A block of the attention leaves at most one
 // segment unfinished behind it, so the grid is over the blocks of the attention
-// or over the segments, whichever are fewer (512 segments on 296 blocks: 29 us
-// in all, over the segments 32; one segment: 9.5 and 8.6).  Further blocks add the
+// or over the segments, whichever are fewer (bf16, 32/8 heads x 128: 64 of up to 512
+// rows, 512 segments on 296 blocks, 29.0 us in all, over the segments 31.8; one
+// of 16,385 rows, 8 segments, 21.3, over the blocks 22.3).  Further blocks add the
 // weights of this step to their accumulators, over the query heads of a
 // key/value head in their order.  Both are short of work and bound by latency
 // (a block of the attention itself that joined 148 parts took 7 us more), so the
@@ -638,11 +640,11 @@ cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t s) {
   if (p.batch == 0) return cudaSuccess;
   const int pairs = p.batch * p.geom.kv_heads;
   // Threads of a block: 1024, or 256 where a thread then has 16 positions at
-  // most; eight such blocks on an SM hide each other's waits (450 pairs of 400
-  // rows: 11 us; with 1024 threads 31).  Blocks of a pair's cluster: doubled while each keeps 2048
-  // positions and the clusters of 1024 threads find room at once, at 96 blocks
-  // (8 pairs of 65,537 rows: 70 us alone, 39 with 4, 30 with 8; 20 pairs of
-  // 25,551: 44 us alone, 23 with 4, but 49 with 8, in two waves).
+  // most; eight such blocks on an SM hide each other's waits (75 x 6 pairs of up to 400
+  // rows of 32, cut to 23: 11.7 us; with 1024 threads 21.8).  Blocks of a pair's cluster: doubled
+  // while each keeps 2048 positions and the clusters of 1024 threads find room at once, at 96 blocks
+  // (1 x 8 pairs of 65,537 rows of 128, cut to 4097: 73 us alone, 42 with 4, 37 with 8; 5 x 4
+  // pairs of 25,551 rows of 64, cut to 1024: 50 us alone, 27 with 4, but 39 with 8, in two waves).
   const bool small = p.max_len <= 4096;
   int cluster = 1;
   while (!small && cluster < kMostBlocks && pairs * cluster * 2 <= 96 && p.max_len / (cluster * 2) >= 2048) cluster *= 2;
