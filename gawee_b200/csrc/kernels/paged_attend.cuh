@@ -360,8 +360,8 @@ struct LaneTile {
 // over fp32's whole range.  fp16 ends at 2^-24, so 2^15 p is split (at most
 // 32768 of 65504) and the sums of values are scaled back at the end: relative error
 // 2^-21, and 2^-40 of the largest weight where that is more.  (Split as it is, p
-// would be lost below 2^-25: 8192 keys 17.4 below one score kept three
-// quarters of their share, 32 keys nothing.)  The sum of the weights takes p itself.
+// would be lost below 2^-25: of 32 keys 17.4 below one score nothing would be
+// left.)  The sum of the weights takes p itself.
 // With up to eight heads hi takes rows 0-7 and lo rows 8-15 of the
 // same product.  D is padded to DT in shared memory; rows are swizzled by 16-byte
 // chunks so that ldmatrix reads eight rows without bank conflicts.
